@@ -76,6 +76,52 @@ int lbm_hip_linear_ss(const lbm_hip_linear_ss_desc* d, lbm_stream_t stream);
 int lbm_hip_layernorm(const float* X, const float* gamma, const float* beta, float* Y, int32_t rows,
                       const uint8_t* keep, const float* fallback, float* Yn, lbm_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Training: the residual join of every block, norm(x + dropout(f(x))) (transformer.py:272-338, msdeformattn.py:185,
+ * nn.Dropout / nn.LayerNorm), forward and backward, for rows of any length in fp32, f16 or bf16.
+ *
+ * Dropout mask.  Element e (row-major index in the logical tensor) lies in block e / 8, slot e % 8.  The four words of
+ * Philox4x32-10(counter = (2 * block + part, offset), key = seed) (Salmon et al., SC 2011; 64-bit halves, low word first) hold
+ * eight 16-bit numbers, slot 2 i in the low half of word i; part 0 gives the upper and part 1 the lower half of each element's
+ * 32-bit number r.  Kept iff r >= round(p * 2^32).  The mask depends on (seed, offset, e) alone: not on type, strides or kernel, so the
+ * backward pass draws it again.  seed_dev != NULL: the 64-bit seed is read from that device word when the kernel runs (a
+ * replayed graph draws new masks when the word changes).  A kept value is multiplied by 1 / (1 - p), a dropped one is 0 whatever it was.     */
+#define LBM_TYPE_F32 0
+#define LBM_TYPE_F16 1
+#define LBM_TYPE_BF16 2
+
+/* y[i] = kept(i) ? x[i] / (1 - p) : 0 for i < n, dense; y may be x.  The gradient of dropout is this call on dy.            */
+int lbm_hip_dropout(const void* x, void* y, int64_t n, int32_t type, double p, uint64_t seed, const void* seed_dev, uint64_t offset,
+                    lbm_stream_t stream);
+
+/* z = x (residual == NULL) or residual + dropout(x);  y = (z - mean(z)) * rstd * weight + bias per row,
+ * rstd = 1 / sqrt(mean((z - mean)^2) + eps).  Statistics and sums are fp32.  Types: x and dx x_type; residual, y, dy and dresidual
+ * res_type (= x_type, or LBM_TYPE_F32: half-precision products beside an fp32 residual stream; without a residual = x_type);
+ * weight, bias and their gradients param_type (= x_type or LBM_TYPE_F32), either may be NULL.  Element strides between rows:
+ * ld_x, ld_residual, ld_dy (>= cols); outputs are dense.  1 <= cols <= 2^28.
+ *
+ * forward: reads x, residual, weight, bias; writes y, and mean / rstd (fp32 [rows], both or neither).
+ * backward: reads dy, x, residual, weight, mean, rstd; writes the non-NULL ones of dx, dresidual, dweight, dbias
+ *   (g = dy * weight; dz = rstd * (g - mean(g) - xhat * mean(g * xhat)); dresidual = dz; dx = dropout's gradient of dz, or dz;
+ *   dweight = sum over rows of dy * xhat, dbias = sum over rows of dy).  z is rebuilt from x, residual and the mask.
+ *   workspace: lbm_hip_norm_workspace_bytes(rows, cols), 16-byte aligned, needed with dweight or dbias; its contents are not kept.
+ *   The sums over rows are made in an order that only the sizes decide: the same call gives the same bits.                     */
+typedef struct {
+  const void* x; const void* residual; const void* weight; const void* bias;
+  void* y; float* mean; float* rstd;
+  const void* dy; void* dx; void* dresidual; void* dweight; void* dbias;
+  void* workspace; uint64_t workspace_bytes;
+  int64_t rows, cols, ld_x, ld_residual, ld_dy;
+  int32_t x_type, res_type, param_type;
+  float eps;
+  double p;                       /* with a residual only; 0: nothing is dropped */
+  uint64_t seed, offset;
+  const void* seed_dev;
+} lbm_hip_norm_desc;
+int lbm_hip_norm_forward(const lbm_hip_norm_desc* d, lbm_stream_t stream);
+int lbm_hip_norm_backward(const lbm_hip_norm_desc* d, lbm_stream_t stream);
+uint64_t lbm_hip_norm_workspace_bytes(int64_t rows, int64_t cols);   /* 0: bad sizes */
+
 /* Y = X / max(|X|_2, 1e-12) per 256-channel row.  Replaces F.normalize (transformer.py:207-212). */
 int lbm_hip_l2norm(const float* X, int64_t ldx, float* Y, int64_t ldy, int64_t rows, lbm_stream_t stream);
 

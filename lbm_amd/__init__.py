@@ -2,11 +2,12 @@
 
 The public surface mirrors the reference (``LBM``, ``LBM_online``, ``LBMTransformer``, ``Backbone``,
 ``MultiScaleDeformableAttention``); the ``lbm`` package next to this one re-exports it under the reference's
-import paths so ``tools/*.py`` run unchanged.  All arithmetic is in ``liblbm_hip.so`` (see ``include/lbm_hip.h``).
+import paths so ``tools/*.py`` run unchanged.  ``layer_norm``, ``dropout`` and ``dropout_add_layer_norm`` are differentiable (``training.py``).  All arithmetic is in ``liblbm_hip.so`` (see ``include/lbm_hip.h``).
 """
 from .config import LBMConfig  # noqa: F401
 
-__all__ = ["LBMConfig", "LBM", "LBM_online", "LBMTransformer", "Backbone", "MultiScaleDeformableAttention"]
+__all__ = ["LBMConfig", "LBM", "LBM_online", "LBMTransformer", "Backbone", "MultiScaleDeformableAttention",
+           "layer_norm", "dropout", "dropout_add_layer_norm"]
 
 
 def __getattr__(name):
@@ -25,4 +26,7 @@ def __getattr__(name):
     if name == "MultiScaleDeformableAttention":
         from .msdeformattn import MultiScaleDeformableAttention
         return MultiScaleDeformableAttention
+    if name in ("layer_norm", "dropout", "dropout_add_layer_norm"):
+        from . import training
+        return getattr(training, name)
     raise AttributeError(name)

@@ -18,6 +18,7 @@
 #include "msda.hpp"
 #include "pyramid.hpp"
 #include "rows.hpp"
+#include "train.hpp"
 
 namespace lbm {
 
@@ -743,6 +744,72 @@ int lbm_hip_split_planes(const float* x, void* hi, void* lo, int64_t n, lbm_stre
 int lbm_hip_layernorm(const float* X, const float* gamma, const float* beta, float* Y, int32_t rows, const uint8_t* keep,
                       const float* fallback, float* Yn, lbm_stream_t stream) {
   return layernorm_rows(X, gamma, beta, Y, rows, keep, fallback, Yn, (hipStream_t)stream);
+}
+
+static bool norm_type_ok(int t) { return t == LBM_TYPE_F32 || t == LBM_TYPE_F16 || t == LBM_TYPE_BF16; }
+// what both passes ask of a descriptor
+static int norm_args(const char* what, const lbm_hip_norm_desc* d, NormArgs& a) {
+  LBM_REQUIRE(d != nullptr, "%s: null descriptor", what);
+  LBM_REQUIRE(d->rows >= 0 && d->cols >= 1 && d->cols <= (1ll << 28) && d->rows <= (1ll << 48) / d->cols, "%s: bad sizes (%lld rows of %lld)", what, (long long)d->rows, (long long)d->cols);
+  LBM_REQUIRE(norm_type_ok(d->x_type) && norm_type_ok(d->res_type) && norm_type_ok(d->param_type), "%s: unknown element type", what);
+  const bool joined = d->residual != nullptr || d->rows == 0;       // a tensor without elements has no address
+  LBM_REQUIRE(d->res_type == d->x_type || (joined && d->res_type == LBM_TYPE_F32), "%s: res_type must be x_type, or fp32 with a residual", what);
+  LBM_REQUIRE(d->param_type == d->x_type || d->param_type == LBM_TYPE_F32, "%s: param_type must be x_type or fp32", what);
+  LBM_REQUIRE(d->rows == 0 || d->x != nullptr, "%s: null x", what);
+  LBM_REQUIRE(d->ld_x >= d->cols && (d->residual == nullptr || d->ld_residual >= d->cols), "%s: a row stride is shorter than a row", what);
+  LBM_REQUIRE(d->eps >= 1.17549435e-38f && d->eps <= 3.402823466e38f, "%s: eps must be a positive normal fp32 number", what);
+  LBM_REQUIRE(joined || d->p == 0.0, "%s: dropout needs a residual to be added to", what);
+  if (make_drop(d->p, d->seed, d->seed_dev, d->offset, a.drop)) return -1;
+  a.x = d->x; a.residual = d->residual; a.weight = d->weight; a.bias = d->bias; a.y = d->y; a.mean = d->mean; a.rstd = d->rstd;
+  a.dy = d->dy; a.dx = d->dx; a.dresidual = d->dresidual; a.dweight = d->dweight; a.dbias = d->dbias;
+  a.workspace = (float*)d->workspace; a.workspace_bytes = d->workspace_bytes;
+  a.rows = d->rows; a.cols = d->cols; a.ld_x = d->ld_x; a.ld_r = d->ld_residual; a.ld_dy = d->ld_dy;
+  a.x_type = d->x_type; a.y_type = d->res_type; a.p_f32 = d->param_type == LBM_TYPE_F32; a.eps = d->eps;
+  const uintptr_t mx = elem_size(a.x_type) - 1, my = elem_size(a.y_type) - 1, mp = elem_size(d->param_type) - 1;
+  LBM_REQUIRE((((uintptr_t)a.x | (uintptr_t)a.dx) & mx) == 0 && (((uintptr_t)a.residual | (uintptr_t)a.y | (uintptr_t)a.dy | (uintptr_t)a.dresidual) & my) == 0 &&
+              (((uintptr_t)a.weight | (uintptr_t)a.bias | (uintptr_t)a.dweight | (uintptr_t)a.dbias) & mp) == 0 &&
+              (((uintptr_t)a.mean | (uintptr_t)a.rstd) & 3) == 0, "%s: a pointer is not aligned to its elements", what);
+  return 0;
+}
+
+int lbm_hip_dropout(const void* x, void* y, int64_t n, int32_t type, double p, uint64_t seed, const void* seed_dev, uint64_t offset,
+                    lbm_stream_t stream) {
+  LBM_REQUIRE(n >= 0 && n < (1ll << 48), "dropout: bad size %lld", (long long)n);
+  LBM_REQUIRE(norm_type_ok(type), "dropout: unknown element type %d", type);
+  DropArgs d;
+  if (make_drop(p, seed, seed_dev, offset, d)) return -1;
+  if (n == 0) return 0;
+  LBM_REQUIRE(x != nullptr && y != nullptr, "dropout: null argument");
+  LBM_REQUIRE((((uintptr_t)x | (uintptr_t)y) & (uintptr_t)(elem_size(type) - 1)) == 0, "dropout: a pointer is not aligned to its elements");
+  return dropout(x, y, n, type, d, (hipStream_t)stream);
+}
+
+int lbm_hip_norm_forward(const lbm_hip_norm_desc* d, lbm_stream_t stream) {
+  NormArgs a;
+  if (norm_args("norm_forward", d, a)) return -1;
+  if (a.rows == 0) return 0;
+  LBM_REQUIRE(a.y != nullptr, "norm_forward: null y");
+  LBM_REQUIRE((a.mean == nullptr) == (a.rstd == nullptr), "norm_forward: mean and rstd go together");
+  return norm_forward(a, (hipStream_t)stream);
+}
+
+int lbm_hip_norm_backward(const lbm_hip_norm_desc* d, lbm_stream_t stream) {
+  NormArgs a;
+  if (norm_args("norm_backward", d, a)) return -1;
+  LBM_REQUIRE(a.rows == 0 || (a.dy != nullptr && a.mean != nullptr && a.rstd != nullptr), "norm_backward: null dy, mean or rstd");
+  LBM_REQUIRE(d->ld_dy >= d->cols, "norm_backward: a row stride is shorter than a row");
+  LBM_REQUIRE(a.dresidual == nullptr || a.residual != nullptr, "norm_backward: dresidual without a residual");
+  if (a.dweight != nullptr || a.dbias != nullptr) {
+    LBM_REQUIRE(a.workspace != nullptr && ((uintptr_t)a.workspace & 15) == 0 && a.workspace_bytes >= norm_workspace_bytes(a.rows, a.cols),
+                "norm_backward: workspace of %llu bytes, %llu needed (16-byte aligned)", (unsigned long long)a.workspace_bytes,
+                (unsigned long long)norm_workspace_bytes(a.rows, a.cols));
+  }
+  return norm_backward(a, (hipStream_t)stream);
+}
+
+uint64_t lbm_hip_norm_workspace_bytes(int64_t rows, int64_t cols) {
+  if (rows < 0 || cols < 1 || cols > (1ll << 28) || rows > (1ll << 48) / cols) return 0;
+  return norm_workspace_bytes(rows, cols);
 }
 
 int lbm_hip_l2norm(const float* X, int64_t ldx, float* Y, int64_t ldy, int64_t rows, lbm_stream_t stream) {

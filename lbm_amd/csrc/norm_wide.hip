@@ -1,0 +1,226 @@
+// Layer normalisation of rows of any length, forward and backward: a workgroup walks a row in several sweeps (the later ones find it in
+// L2) and the gradients of weight and bias are summed by a kernel of their own that owns columns.
+//   z = residual + dropout(x);  m = mean(z);  v = mean((z - m)^2);  rstd = 1 / sqrt(v + eps);  xhat = (z - m) rstd;  y = xhat w + b
+//   g = dy w;  dz = rstd (g - mean(g) - xhat mean(g xhat));  dresidual = dz;  dx = keep ? dz scale : 0
+//   dw = sum over rows of dy xhat;  db = sum over rows of dy
+// All sums are fp32.  z is rebuilt from x, residual and the mask in the backward pass: storing it would move the same bytes (one write
+// and one read against two reads for one), round it, and hold one more tensor.
+#include "train.hpp"
+
+namespace lbm {
+
+// the eight z values of a chunk, and the mask bits when something is dropped
+template <class TX, class TR, int RES>
+__device__ __forceinline__ uint32_t load_z(const NormArgs& a, const DropKey& key, long long row, long long c, int nv, float (&z)[8]) {
+  Vec8<TX> vx;
+  vx.load(reinterpret_cast<const TX*>(a.x) + row * a.ld_x + c, nv);
+  uint32_t m = 0xffu;
+  Vec8<TR> vr;
+  float scale = 1.0f;
+  if (RES) {
+    vr.load(reinterpret_cast<const TR*>(a.residual) + row * a.ld_r + c, nv);
+    if (a.drop.on) {
+      m = keep8((uint64_t)(row * a.cols + c), key, a.drop.tm1);
+      scale = a.drop.scale;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) z[j] = join_one<RES>(vx.get(j), RES ? vr.get(j) : 0.0f, m >> j & 1, scale);
+  return m;
+}
+
+template <class TX, class TR, int RES>
+__global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
+  __shared__ float sm[2][16];
+  DropKey key{};
+  if (RES) key = drop_key(a.drop);
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    float s = 0.0f, z[8];
+    for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
+      const int nv = (int)min(8ll, a.cols - c);
+      load_z<TX, TR, RES>(a, key, row, c, nv, z);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += j < nv ? z[j] : 0.0f;
+    }
+    const float mean = block_sum(s, sm[0]) / (float)a.cols;
+    s = 0.0f;
+    for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
+      const int nv = (int)min(8ll, a.cols - c);
+      load_z<TX, TR, RES>(a, key, row, c, nv, z);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += j < nv ? (z[j] - mean) * (z[j] - mean) : 0.0f;
+    }
+    const float rstd = 1.0f / sqrtf(block_sum(s, sm[1]) / (float)a.cols + a.eps);
+    if (threadIdx.x == 0 && a.mean != nullptr) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+    for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
+      const int nv = (int)min(8ll, a.cols - c);
+      float w[8], b[8];
+      load_z<TX, TR, RES>(a, key, row, c, nv, z);
+      load_param<TX>(a.weight, a.p_f32, c, nv, 1.0f, w);
+      load_param<TX>(a.bias, a.p_f32, c, nv, 0.0f, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[j] = fmaf((z[j] - mean) * rstd, w[j], b[j]);
+      Vec8<TR> o;
+      o.set(z);
+      o.store(reinterpret_cast<TR*>(a.y) + row * a.cols + c, nv);
+    }
+  }
+}
+
+template <class TX, class TR, int RES>
+__global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
+  __shared__ float sm[2][16];
+  DropKey key{};
+  if (RES) key = drop_key(a.drop);
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float s1 = 0.0f, s2 = 0.0f, z[8], w[8];
+    for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
+      const int nv = (int)min(8ll, a.cols - c);
+      load_z<TX, TR, RES>(a, key, row, c, nv, z);
+      load_param<TX>(a.weight, a.p_f32, c, nv, 1.0f, w);
+      Vec8<TR> d;
+      d.load(reinterpret_cast<const TR*>(a.dy) + row * a.ld_dy + c, nv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float g = d.get(j) * w[j];
+        s1 += j < nv ? g : 0.0f;
+        s2 += j < nv ? g * ((z[j] - mean) * rstd) : 0.0f;
+      }
+    }
+    const float c1 = block_sum(s1, sm[0]) / (float)a.cols, c2 = block_sum(s2, sm[1]) / (float)a.cols;
+    for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
+      const int nv = (int)min(8ll, a.cols - c);
+      const uint32_t m = load_z<TX, TR, RES>(a, key, row, c, nv, z);
+      load_param<TX>(a.weight, a.p_f32, c, nv, 1.0f, w);
+      Vec8<TR> d;
+      d.load(reinterpret_cast<const TR*>(a.dy) + row * a.ld_dy + c, nv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[j] = rstd * (d.get(j) * w[j] - c1 - (z[j] - mean) * rstd * c2);
+      if (RES && a.dresidual != nullptr) {
+        d.set(z);
+        d.store(reinterpret_cast<TR*>(a.dresidual) + row * a.cols + c, nv);
+      }
+      if (a.dx != nullptr) {
+        if (RES && a.drop.on) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) z[j] = (m >> j & 1) ? z[j] * a.drop.scale : 0.0f;
+        }
+        Vec8<TX> o;
+        o.set(z);
+        o.store(reinterpret_cast<TX*>(a.dx) + row * a.cols + c, nv);
+      }
+    }
+  }
+}
+
+// partial[g][0 / 1][cols]: sums of dy xhat and of dy over the rows g, g + G, ...; a thread owns eight columns
+template <class TX, class TR, int RES>
+__global__ __launch_bounds__(256) void norm_wide_dw_kernel(NormArgs a) {
+  DropKey key{};
+  if (RES) key = drop_key(a.drop);
+  const long long c = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (c >= a.cols) return;
+  const int nv = (int)min(8ll, a.cols - c);
+  float dw[8] = {}, db[8] = {}, z[8];
+  for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    load_z<TX, TR, RES>(a, key, row, c, nv, z);
+    Vec8<TR> d;
+    d.load(reinterpret_cast<const TR*>(a.dy) + row * a.ld_dy + c, nv);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      dw[j] = fmaf(d.get(j), (z[j] - mean) * rstd, dw[j]);
+      db[j] += d.get(j);
+    }
+  }
+  float* p = a.workspace + (long long)blockIdx.y * 2 * a.cols + c;
+  for (int j = 0; j < nv; ++j) {
+    p[j] = dw[j];
+    p[a.cols + j] = db[j];
+  }
+}
+
+// dweight / dbias = the partial sums added up in a fixed order; 16 columns x 16 slices of the partials a workgroup
+template <class T>
+__global__ __launch_bounds__(256) void norm_dw_finish_kernel(const float* part, int parts, long long cols, T* dweight, T* dbias) {
+  __shared__ float sm[16][17];
+  const int tc = threadIdx.x & 15, tg = threadIdx.x >> 4;
+  const long long c = (long long)blockIdx.x * 16 + tc;              // over 2 cols: dweight, then dbias
+  float s = 0.0f;
+  if (c < 2 * cols)
+    for (int g = tg; g < parts; g += 16) s += part[(long long)g * 2 * cols + c];
+  sm[tg][tc] = s;
+  __syncthreads();
+  if (tg == 0 && c < 2 * cols) {
+    s = 0.0f;
+#pragma unroll
+    for (int g = 0; g < 16; ++g) s += sm[g][tc];
+    T* o = c < cols ? dweight : dbias;
+    if (o != nullptr) o[c < cols ? c : c - cols] = (T)s;
+  }
+}
+
+static int wide_parts(long long rows, long long cols) {
+  const long long slabs = (cols + 2047) / 2048;                     // workgroups along the columns; fill ~1024 with rows
+  long long g = (1024 + slabs - 1) / slabs;
+  if (g > rows) g = rows;
+  return (int)(g < 1 ? 1 : g);
+}
+
+uint64_t norm_workspace_bytes(long long rows, long long cols) { return (uint64_t)wide_parts(rows, cols) * 2 * (uint64_t)cols * sizeof(float); }
+
+template <class TX, class TR, int RES> static int wide_forward(const NormArgs& a, hipStream_t s) {
+  const unsigned grid = (unsigned)(a.rows < (1ll << 30) ? a.rows : (1ll << 30));
+  norm_wide_fwd_kernel<TX, TR, RES><<<grid, 256, 0, s>>>(a);
+  return check_launch("norm_forward");
+}
+template <class TX, class TR, int RES> static int wide_backward(const NormArgs& a, hipStream_t s) {
+  if (a.rows > 0 && (a.dx != nullptr || a.dresidual != nullptr)) {
+    const unsigned grid = (unsigned)(a.rows < (1ll << 30) ? a.rows : (1ll << 30));
+    norm_wide_dx_kernel<TX, TR, RES><<<grid, 256, 0, s>>>(a);
+    if (check_launch("norm_backward")) return -1;
+  }
+  if (a.dweight != nullptr || a.dbias != nullptr) {
+    const int parts = wide_parts(a.rows, a.cols);
+    norm_wide_dw_kernel<TX, TR, RES><<<dim3((unsigned)((a.cols + 2047) / 2048), parts), 256, 0, s>>>(a);
+    if (check_launch("norm_backward")) return -1;
+    const unsigned fin = (unsigned)((2 * a.cols + 15) / 16);
+    if (a.p_f32)
+      norm_dw_finish_kernel<float><<<fin, 256, 0, s>>>(a.workspace, parts, a.cols, (float*)a.dweight, (float*)a.dbias);
+    else
+      norm_dw_finish_kernel<TX><<<fin, 256, 0, s>>>(a.workspace, parts, a.cols, (TX*)a.dweight, (TX*)a.dbias);
+    return check_launch("norm_backward");
+  }
+  return 0;
+}
+
+// calls f<TX, TR, RES>(a, s) for the types of a
+#define NORM_DISPATCH(F, a, s)                                                                            \
+  do {                                                                                                    \
+    if (a.residual == nullptr) {                                                                          \
+      if (a.x_type == kF32) return F<float, float, 0>(a, s);                                              \
+      if (a.x_type == kF16) return F<_Float16, _Float16, 0>(a, s);                                        \
+      return F<__bf16, __bf16, 0>(a, s);                                                                  \
+    }                                                                                                     \
+    if (a.x_type == kF32) return F<float, float, 1>(a, s);                                                \
+    if (a.x_type == kF16) return a.y_type == kF32 ? F<_Float16, float, 1>(a, s) : F<_Float16, _Float16, 1>(a, s); \
+    return a.y_type == kF32 ? F<__bf16, float, 1>(a, s) : F<__bf16, __bf16, 1>(a, s);                     \
+  } while (0)
+
+int norm_forward(const NormArgs& a, hipStream_t stream) {
+  if (a.rows == 0) return 0;
+  ProfScope prof("norm_forward", stream, 8.0 * a.rows * a.cols,
+                 (double)a.rows * a.cols * (elem_size(a.x_type) + elem_size(a.y_type) * (a.residual ? 2.0 : 1.0)));
+  NORM_DISPATCH(wide_forward, a, stream);
+}
+int norm_backward(const NormArgs& a, hipStream_t stream) {
+  ProfScope prof("norm_backward", stream, 14.0 * a.rows * a.cols,
+                 (double)a.rows * a.cols * (2.0 * elem_size(a.x_type) + elem_size(a.y_type) * (a.residual ? 3.0 : 1.0)));
+  NORM_DISPATCH(wide_backward, a, stream);
+}
+
+}  // namespace lbm

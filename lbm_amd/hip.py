@@ -7,6 +7,7 @@ PyTorch/CPU fallback — if the library is missing or no GPU is present the call
 from __future__ import annotations
 
 import ctypes as C
+import operator
 import os
 import re
 from pathlib import Path
@@ -31,6 +32,7 @@ EXPORTS = (
     "lbm_hip_debug_ptr", "lbm_hip_update_points_static", "lbm_hip_preprocess_u8", "lbm_hip_corr_topk",
     "lbm_hip_corr_topk_workspace_bytes", "lbm_hip_preprocess_split", "lbm_hip_stem_pool",
     "lbm_hip_encoder_tail_fused", "lbm_hip_debug_active", "lbm_hip_tuning_build", "lbm_hip_attn_readout_h16",
+    "lbm_hip_dropout", "lbm_hip_norm_forward", "lbm_hip_norm_backward", "lbm_hip_norm_workspace_bytes",
 )
 
 
@@ -88,6 +90,16 @@ class StepDesc(C.Structure):
                 ("phase", C.c_int32), ("row_lo", C.c_int32), ("row_count", C.c_int32), ("sub_index", C.c_int32),
                 ("query_split", C.c_void_p), ("vis_flag", C.c_void_p), ("rho_prob", C.c_void_p),
                 ("query_u0", C.c_void_p), ("query_u0_valid", C.c_int32), ("inv_norm", C.c_void_p)]
+
+
+class NormDesc(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("residual", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p),
+                ("y", C.c_void_p), ("mean", C.c_void_p), ("rstd", C.c_void_p),
+                ("dy", C.c_void_p), ("dx", C.c_void_p), ("dresidual", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+                ("rows", C.c_int64), ("cols", C.c_int64), ("ld_x", C.c_int64), ("ld_residual", C.c_int64), ("ld_dy", C.c_int64),
+                ("x_type", C.c_int32), ("res_type", C.c_int32), ("param_type", C.c_int32), ("eps", C.c_float),
+                ("p", C.c_double), ("seed", C.c_uint64), ("offset", C.c_uint64), ("seed_dev", C.c_void_p)]
 
 
 class ProfileEntry(C.Structure):
@@ -176,6 +188,11 @@ def load() -> C.CDLL:
     lib.lbm_hip_corr_topk_workspace_bytes.argtypes = [C.c_int32] * 4
     lib.lbm_hip_corr_topk.argtypes = [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                       C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.lbm_hip_dropout.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_double, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p]
+    lib.lbm_hip_norm_forward.argtypes = [C.POINTER(NormDesc), C.c_void_p]
+    lib.lbm_hip_norm_backward.argtypes = [C.POINTER(NormDesc), C.c_void_p]
+    lib.lbm_hip_norm_workspace_bytes.restype = C.c_uint64
+    lib.lbm_hip_norm_workspace_bytes.argtypes = [C.c_int64, C.c_int64]
     _lib = lib
     return lib
 
@@ -526,6 +543,151 @@ def l2norm(x: torch.Tensor) -> torch.Tensor:
     rows = x.numel() // 256
     _check(load().lbm_hip_l2norm(_p(x), 256, _p(y), 256, rows, _stream()), "lbm_hip_l2norm")
     return y
+
+
+# ---- training operators (differentiable forms: lbm_amd/training.py) ----
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}       # LBM_TYPE_*
+
+
+def _elem_type(t: torch.Tensor, what: str) -> int:
+    if not t.is_cuda:
+        raise HipError(f"{what}: expected a GPU tensor")
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        raise HipError(f"{what}: expected float32, float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _as_rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """(t, elements between rows): rows of the last dimension at one stride are used where they lie, any other layout is copied."""
+    n = t.shape[-1]
+    if t.is_contiguous():
+        return t, n
+    shape, stride = t.shape, t.stride()
+    if stride[-1] == 1 and t.numel():
+        rows = [(s, d) for s, d in zip(shape[:-1], stride[:-1]) if s != 1]
+        if all(rows[i][1] == rows[i + 1][1] * rows[i + 1][0] for i in range(len(rows) - 1)):
+            ld = rows[-1][1] if rows else n
+            if ld >= n:
+                return t, ld
+    return t.contiguous(), n
+
+
+def _drop_args(p, seed, offset, device, what: str):
+    """-> (p, seed value, its device pointer, offset) of a dropout mask; seed: an integer or an int64 GPU tensor of one element."""
+    p, offset = float(p), operator.index(offset)
+    if not 0.0 <= p <= 1.0:
+        raise HipError(f"{what}: p = {p} is not a probability")
+    if not 0 <= offset < 1 << 64:
+        raise HipError(f"{what}: offset {offset} is outside 0 .. 2^64 - 1")
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
+            raise HipError(f"{what}: a seed tensor holds one int64 on the operands' device")
+        return p, 0, seed.data_ptr(), offset
+    seed = operator.index(seed)
+    if not -(1 << 63) <= seed < 1 << 64:
+        raise HipError(f"{what}: seed {seed} does not fit 64 bits")
+    return p, seed & 0xFFFFFFFFFFFFFFFF, None, offset
+
+
+def _call_on(device: torch.device, fn, what: str, *args) -> None:
+    """fn(*args, stream) on the current stream of the operands' device, whichever device is the current one."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc != 0:
+        _check(rc, what)
+
+
+def dropout(x: torch.Tensor, p: float, seed, offset: int = 0) -> torch.Tensor:
+    """x / (1 - p) where the mask of (seed, offset) keeps an element, else 0 (lbm_hip_dropout); dense result.  On dy: the gradient."""
+    code = _elem_type(x, "dropout")
+    p, seed_value, seed_dev, offset = _drop_args(p, seed, offset, x.device, "dropout")
+    x = x.contiguous()
+    y = torch.empty_like(x)
+    _call_on(x.device, load().lbm_hip_dropout, "lbm_hip_dropout", x.data_ptr(), y.data_ptr(), x.numel(), code, p, seed_value, seed_dev, offset)
+    return y
+
+
+def _norm_operands(what: str, x, residual, weight, bias):
+    """Checks shared by both passes -> (x, ld_x, residual, ld_residual, weight, bias, x_type, res_type, param_type)."""
+    tx = tr = tp = _elem_type(x, what)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise HipError(f"{what}: x needs a last dimension of at least one element, got shape {tuple(x.shape)}")
+    dev, ldr = x.device, 0
+    x, ldx = _as_rows(x)
+    if residual is not None:
+        tr = _elem_type(residual, what)
+        if residual.shape != x.shape or residual.device != dev:
+            raise HipError(f"{what}: residual has shape {tuple(residual.shape)} on {residual.device}, x {tuple(x.shape)} on {dev}")
+        if tr != tx and tr != 0:
+            raise HipError(f"{what}: the residual's type must be x's ({x.dtype}) or float32, got {residual.dtype}")
+        residual, ldr = _as_rows(residual)
+    given = [t for t in (weight, bias) if t is not None]
+    for t in given:
+        tp = _elem_type(t, what)
+        if t.shape != x.shape[-1:] or t.device != dev:
+            raise HipError(f"{what}: weight / bias have shape {tuple(t.shape)} on {t.device}, expected ({x.shape[-1]},) on {dev}")
+        if tp != tx and tp != 0:
+            raise HipError(f"{what}: the type of weight and bias must be x's ({x.dtype}) or float32, got {t.dtype}")
+    if len(given) == 2 and weight.dtype != bias.dtype:
+        raise HipError(f"{what}: weight and bias differ in type ({weight.dtype}, {bias.dtype})")
+    return (x, ldx, residual, ldr, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), tx, tr, tp)
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float = 1e-5,
+                 residual: Optional[torch.Tensor] = None, p: float = 0.0, seed=0, offset: int = 0, want_stats: bool = False):
+    """layer_norm of x, or of residual + dropout(x) (lbm_hip_norm_forward) -> y in the residual's type (x's without one), dense;
+    with want_stats (y, mean, rstd): what norm_backward needs beside the inputs."""
+    x, ldx, residual, ldr, weight, bias, tx, tr, tp = _norm_operands("norm_forward", x, residual, weight, bias)
+    p, seed_value, seed_dev, offset = _drop_args(p, seed, offset, x.device, "norm_forward")
+    cols = x.shape[-1]
+    rows = x.numel() // cols
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype if residual is None else residual.dtype)
+    mean = rstd = None
+    if want_stats:
+        mean, rstd = torch.empty(2, rows, device=x.device, dtype=torch.float32).unbind(0)
+    d = NormDesc(x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(mean), _ptr(rstd), None, None, None, None, None,
+                 None, 0, rows, cols, ldx, ldr, 0, tx, tr, tp, eps, p, seed_value, offset, seed_dev)
+    _call_on(x.device, load().lbm_hip_norm_forward, "lbm_hip_norm_forward", C.byref(d))
+    return (y, mean, rstd) if want_stats else y
+
+
+def norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: Optional[torch.Tensor],
+                  bias: Optional[torch.Tensor] = None, eps: float = 1e-5, residual: Optional[torch.Tensor] = None, p: float = 0.0, seed=0,
+                  offset: int = 0, want: Sequence[bool] = (True, True, True, True)):
+    """Gradients of norm_forward at dy (lbm_hip_norm_backward) -> (dx, dresidual, dweight, dbias), None where `want` is false or the
+    operand is absent.  The arguments are the forward call's; mean and rstd its statistics."""
+    x, ldx, residual, ldr, weight, bias, tx, tr, tp = _norm_operands("norm_backward", x, residual, weight, bias)
+    p, seed_value, seed_dev, offset = _drop_args(p, seed, offset, x.device, "norm_backward")
+    dev, cols = x.device, x.shape[-1]
+    rows = x.numel() // cols
+    ytype = x.dtype if residual is None else residual.dtype
+    if dy.shape != x.shape or dy.dtype != ytype or dy.device != dev:
+        raise HipError(f"norm_backward: dy has shape {tuple(dy.shape)}, type {dy.dtype}, on {dy.device}; expected {tuple(x.shape)}, {ytype}, on {dev}")
+    for t in (mean, rstd):
+        if t.dtype != torch.float32 or t.numel() != rows or t.device != dev or not t.is_contiguous():
+            raise HipError("norm_backward: mean and rstd are the dense fp32 statistics of norm_forward, one a row")
+    dy, lddy = _as_rows(dy)
+    dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if want[0] else None
+    dres = torch.empty(x.shape, device=dev, dtype=ytype) if want[1] and residual is not None else None
+    dw = torch.empty_like(weight) if want[2] and weight is not None else None
+    db = torch.empty_like(bias) if want[3] and bias is not None else None
+    lib, ws, nbytes = load(), None, 0
+    if dw is not None or db is not None:
+        nbytes = lib.lbm_hip_norm_workspace_bytes(rows, cols)
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    d = NormDesc(x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias), None, mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), _ptr(dx),
+                 _ptr(dres), _ptr(dw), _ptr(db), _ptr(ws), nbytes, rows, cols, ldx, ldr, lddy, tx, tr, tp, eps, p, seed_value, offset, seed_dev)
+    _call_on(dev, lib.lbm_hip_norm_backward, "lbm_hip_norm_backward", C.byref(d))
+    return dx, dres, dw, db
 
 
 def attn_readout(U, seq, S, ring_head=0, temb=None, mask_a=None, mask_b=None, want_valid=False):

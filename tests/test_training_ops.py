@@ -1,0 +1,585 @@
+"""layer_norm, dropout and dropout_add_layer_norm (lbm_amd/training.py) against the float64 / integer oracle.
+
+Error bounds.  u(T) = finfo(T).eps / 2 is one rounding to T, e = 2^-24 one to fp32.  A row's sums are made of at most
+depth(D) = 8 ceil(D / 2048) + 32 dependent fp32 additions (eight a chunk in a thread, a tree over lanes and waves), so a mean is off by
+(depth + 2) e mean|z|, and
+  E = e (depth + 16) rstd (mean|z| + |z| + |x scale|) + e (depth + 16) 2 |xhat|      bounds the error of xhat
+(the first part: mean and the join's own roundings; the second: the variance's sum, square root, division, product).  From there
+  y      u |y| + |w| E + 4 e (|xhat w| + |b|)
+  dz     u |dz| + rstd (4 e |g| + e (depth + 4) mean|g| + |xhat| (e (depth + 4) mean|g xhat| + mean(|g| E)) + E |mean(g xhat)|) + e (depth + 16) |dz|
+  dx     that times scale, its own rounding, and 4 e |dx|
+  dw     u |dw| + sum |dy| E + e n sum |dy xhat|     n = rows summed in sequence, at most rows / 64 + 64 (fewer rows: all), + 32
+  db     u |db| + e n sum |dy|
+and half of the smallest subnormal of f16 where results are that small.
+"""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from lbm_amd import dropout, dropout_add_layer_norm, hip, layer_norm
+from oracle import train_ref as ref
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+E32 = 2.0 ** -24
+gpu = pytest.mark.gpu
+
+
+def u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def tiny(dtype):
+    return 2.0 ** -25 if dtype == F16 else 0.0
+
+
+def bounds(o, eps, dtype_y, dtype_x, dtype_p, scale=1.0):
+    """Tolerances of y, dresidual / dz, dx, dweight, dbias (docstring above)."""
+    D = o["z"].shape[-1]
+    rows = o["z"].numel() // D
+    depth = 8 * math.ceil(D / 2048) + 32
+    mean = lambda t: t.mean(-1, keepdim=True)        # noqa: E731
+    E = E32 * (depth + 16) * (o["rstd"] * (mean(o["z"].abs()) + o["z"].abs() + o["xs"].abs()) + 2 * o["xhat"].abs())
+    t = {"y": u(dtype_y) * o["y"].abs() + o["w"].abs() * E + 4 * E32 * ((o["xhat"] * o["w"]).abs() + o["b"].abs()) + tiny(dtype_y)}
+    if "dy" in o:
+        g, xh, dz = o["g"].abs(), o["xhat"].abs(), o["dresidual"].abs()
+        raw = o["rstd"] * (4 * E32 * g + E32 * (depth + 4) * mean(g) + xh * (E32 * (depth + 4) * mean(g * xh) + mean(g * E)) + E * o["c2"].abs()) \
+            + E32 * (depth + 16) * dz
+        t["dresidual"] = u(dtype_y) * dz + raw + tiny(dtype_y)
+        t["dx"] = u(dtype_x) * o["dx"].abs() + raw * scale + 4 * E32 * o["dx"].abs() + tiny(dtype_x)
+        n = min(rows, rows / 64 + 64) + 32
+        flat = lambda v: v.reshape(-1, D).sum(0)     # noqa: E731
+        t["dweight"] = u(dtype_p) * o["dweight"].abs() + flat(o["dy"].abs() * E) + E32 * n * flat((o["dy"] * o["xhat"]).abs()) + tiny(dtype_p)
+        t["dbias"] = u(dtype_p) * o["dbias"].abs() + E32 * n * flat(o["dy"].abs()) + tiny(dtype_p)
+    return t
+
+
+def within(got, want, tol, what):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    bad = ~((got - want).abs() <= tol)
+    assert not bool(bad.any()), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float(((got - want).abs() / tol.clamp_min(1e-300)).max()):.2f} of the bound"
+
+
+def operands(shape, x_type, res_type, p_type, affine, seed, offset_rows=0.3):
+    g = torch.Generator().manual_seed(seed)
+    D = shape[-1]
+    x = torch.randn(*shape, generator=g) * torch.exp(0.5 * torch.randn(*shape[:-1], 1, generator=g)) + offset_rows * torch.randn(*shape[:-1], 1, generator=g)
+    r = torch.randn(*shape, generator=g)
+    w = 1 + 0.2 * torch.randn(D, generator=g)
+    b = 0.2 * torch.randn(D, generator=g)
+    dy = torch.randn(*shape, generator=g)
+    out = dict(x=x.to(x_type), residual=None if res_type is None else r.to(res_type), weight=w.to(p_type) if affine in ("both", "weight") else None,
+               bias=b.to(p_type) if affine in ("both", "bias") else None, dy=dy.to(res_type or x_type))
+    return {k: None if v is None else v.cuda() for k, v in out.items()}
+
+
+def check(o, p=0.0, seed=0, offset=0, eps=1e-5, x_view=None):
+    """Forward without gradients, then forward and backward, of the operator that the operands ask for."""
+    joined = o["residual"] is not None
+    x = o["x"] if x_view is None else x_view
+    D = x.shape[-1]
+    factor = None
+    if joined and p > 0:
+        factor = ref.keep(tuple(x.shape), p, seed, offset).double() * ref.scale(p)
+    want = ref.norm(x, o["weight"], o["bias"], eps, o["residual"], factor, o["dy"])
+    given = [o[k] for k in ("weight", "bias") if o[k] is not None]
+    tol = bounds(want, eps, o["dy"].dtype, x.dtype, given[0].dtype if given else x.dtype, ref.scale(p) if joined else 1.0)
+
+    def call(x, residual, weight, bias):
+        if joined:
+            return dropout_add_layer_norm(x, residual, weight, bias, p=p, seed=seed, offset=offset, eps=eps)
+        return layer_norm(x, weight, bias, eps)
+
+    plain = call(x, o["residual"], o["weight"], o["bias"])
+    assert plain.dtype == o["dy"].dtype and plain.is_contiguous() and not plain.requires_grad
+    within(plain, want["y"], tol["y"], "y")
+    leaves = {k: (x if k == "x" else o[k]).detach().requires_grad_() for k in ("x", "residual", "weight", "bias") if k == "x" or o[k] is not None}
+    y = call(leaves["x"], leaves.get("residual"), leaves.get("weight"), leaves.get("bias"))
+    assert torch.equal(y.detach().view(torch.uint8) if y.numel() else y, plain.view(torch.uint8) if y.numel() else plain)     # with and without statistics: the same bits
+    grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), o["dy"])))
+    for k, t in grads.items():
+        assert t.dtype == leaves[k].dtype
+        within(t, want["d" + k], tol["d" + k], "d" + k)
+    return want, grads
+
+
+# ---------------------------------------------------------------------------------------------- CPU: the oracle, refusals
+
+def test_oracle_generator_known_answers():
+    """The published test vectors of Philox4x32-10."""
+    f = 0xFFFFFFFF
+    for ctr, key, want in (((0, 0, 0, 0), (0, 0), (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)),
+                           ((f, f, f, f), (f, f), (0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD)),
+                           ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0), (0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1))):
+        assert tuple(int(w) for w in ref.philox4x32(ctr, key)) == want
+
+
+def test_oracle_mask_rate():
+    """Kept elements of 2^20: the count is binomial; 6 standard deviations."""
+    n = 1 << 20
+    for p in (0.1, 0.5, 0.9):
+        k = int(ref.keep((n,), p, 1234, 5).sum())
+        assert abs(k - n * (1 - p)) < 6 * math.sqrt(n * p * (1 - p))
+    assert not torch.equal(ref.keep((n,), 0.5, 1234, 5), ref.keep((n,), 0.5, 1234, 6))
+
+
+def test_oracle_gradients_against_differences():
+    g = torch.Generator().manual_seed(3)
+    D = 7
+    t = {k: torch.randn(*s, generator=g, dtype=torch.float64) for k, s in (("x", (3, D)), ("r", (3, D)), ("w", (D,)), ("b", (D,)), ("dy", (3, D)))}
+    factor = ref.keep((3, D), 0.3, 9, 2).double() * ref.scale(0.3)
+    o = ref.norm(t["x"], t["w"], t["b"], 1e-5, t["r"], factor, t["dy"])
+    loss = lambda: (ref.norm(t["x"], t["w"], t["b"], 1e-5, t["r"], factor)["y"] * t["dy"]).sum()     # noqa: E731
+    for k, name in (("x", "dx"), ("r", "dresidual"), ("w", "dweight"), ("b", "dbias")):
+        v = torch.randn(t[k].shape, generator=g, dtype=torch.float64)
+        keep, h = t[k].clone(), 1e-5
+        t[k] = keep + h * v
+        up = loss()
+        t[k] = keep - h * v
+        down = loss()
+        t[k] = keep
+        assert abs(float((up - down) / (2 * h) - (o[name] * v).sum())) < 1e-8        # h^2 third derivatives (~100) and 1e-16 / h
+
+
+def _desc(**kw):
+    a = torch.zeros(64)
+    d = hip.NormDesc()
+    d.x = d.y = d.dy = d.dx = a.data_ptr()
+    d.mean = d.rstd = a.data_ptr()
+    d.rows, d.cols, d.ld_x, d.ld_residual, d.ld_dy, d.eps = 2, 8, 8, 8, 8, 1e-5
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d, a
+
+
+@pytest.mark.parametrize("kw,message", [
+    (dict(cols=0), b"bad sizes"), (dict(rows=-1), b"bad sizes"), (dict(cols=(1 << 28) + 1, ld_x=1 << 29), b"bad sizes"),
+    (dict(x_type=3), b"element type"), (dict(param_type=-1), b"element type"), (dict(res_type=1), b"res_type"),
+    (dict(x_type=1, res_type=0), b"res_type"), (dict(x_type=1, res_type=1, param_type=2), b"param_type"), (dict(ld_x=7), b"row stride"),
+    (dict(eps=0.0), b"eps"), (dict(eps=float("nan")), b"eps"), (dict(eps=float("inf")), b"eps"), (dict(x=None), b"null x"),
+    (dict(p=0.5), b"residual"), (dict(p=float("nan")), b"residual"), (dict(x=2), b"aligned")])
+def test_abi_refusals_of_both_passes(kw, message):
+    lib = hip.load()
+    d, _keep = _desc(**kw)
+    for fn in (lib.lbm_hip_norm_forward, lib.lbm_hip_norm_backward):
+        assert fn(C.byref(d), None) != 0
+        assert message in lib.lbm_hip_last_error(), lib.lbm_hip_last_error()
+
+
+def test_abi_refusals_of_one_pass():
+    lib = hip.load()
+    assert lib.lbm_hip_norm_forward(None, None) != 0 and b"null descriptor" in lib.lbm_hip_last_error()
+    for kw, msg in ((dict(y=None), b"null y"), (dict(mean=None), b"go together"), (dict(residual=64, p=1.5), b"not a probability"),
+                    (dict(residual=64, ld_residual=4), b"row stride"), (dict(seed_dev=4), b"seed")):
+        d, _keep = _desc(**kw)
+        assert lib.lbm_hip_norm_forward(C.byref(d), None) != 0 and msg in lib.lbm_hip_last_error(), (kw, lib.lbm_hip_last_error())
+    for kw, msg in ((dict(dy=None), b"null dy"), (dict(rstd=None), b"null dy"), (dict(ld_dy=1), b"row stride"), (dict(dresidual=64), b"without a residual"),
+                    (dict(dweight=64), b"workspace"), (dict(dbias=64, workspace=64, workspace_bytes=8), b"workspace"),
+                    (dict(dbias=64, workspace=68, workspace_bytes=1 << 40), b"workspace")):
+        d, _keep = _desc(**kw)
+        assert lib.lbm_hip_norm_backward(C.byref(d), None) != 0 and msg in lib.lbm_hip_last_error(), (kw, lib.lbm_hip_last_error())
+    a = torch.zeros(64)
+    for args, msg in (((a.data_ptr(), a.data_ptr(), -1, 0, 0.5, 1, None, 0), b"bad size"), ((a.data_ptr(), a.data_ptr(), 8, 7, 0.5, 1, None, 0), b"element type"),
+                      ((a.data_ptr(), a.data_ptr(), 8, 0, -0.1, 1, None, 0), b"probability"), ((a.data_ptr(), a.data_ptr(), 8, 0, float("nan"), 1, None, 0), b"probability"),
+                      ((None, a.data_ptr(), 8, 0, 0.5, 1, None, 0), b"null"), ((a.data_ptr() + 2, a.data_ptr(), 8, 0, 0.5, 1, None, 0), b"aligned")):
+        assert lib.lbm_hip_dropout(*args, None) != 0 and msg in lib.lbm_hip_last_error(), lib.lbm_hip_last_error()
+    for bad in ((-1, 8), (1, 0), (1 << 45, 1 << 10), (1, (1 << 28) + 1)):
+        assert lib.lbm_hip_norm_workspace_bytes(*bad) == 0
+    assert lib.lbm_hip_norm_workspace_bytes(0, 8) > 0
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(2, 8)
+    for call in (lambda: layer_norm(x), lambda: dropout(x, 0.5, 1), lambda: dropout_add_layer_norm(x, x)):
+        with pytest.raises(hip.HipError, match="GPU"):
+            call()
+
+
+# ---------------------------------------------------------------------------------------------- dropout
+
+SIZES = [1, 7, 8, 9, 511, 2048, 2049, 100003]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n", SIZES)
+def test_dropout_bits(dtype, n):
+    """The mask and the values, bit for bit: one fp32 product, one rounding."""
+    for k, p in enumerate((0.1, 0.5, 1 / 3, 0.999)):
+        x = torch.randn(n, generator=torch.Generator().manual_seed(n + k)).to(dtype)
+        seed, offset = 0x9E3779B97F4A7C15 * (k + 1) % 2 ** 64, 2 ** 63 + k
+        m = ref.keep((n,), p, seed, offset)
+        want = torch.where(m, x.float() * torch.tensor(ref.scale(p), dtype=F32), torch.zeros(())).to(dtype)
+        leaf = x.cuda().requires_grad_()
+        y = dropout(leaf, p, seed, offset)
+        assert torch.equal(y.detach().cpu(), want)
+        assert torch.equal(dropout(leaf.detach(), p, seed, offset).cpu(), want)
+        dy = torch.randn(n, generator=torch.Generator().manual_seed(n + k + 99)).to(dtype)
+        dx, = torch.autograd.grad(y, leaf, dy.cuda())
+        assert torch.equal(dx.cpu(), torch.where(m, dy.float() * torch.tensor(ref.scale(p), dtype=F32), torch.zeros(())).to(dtype))
+
+
+@gpu
+def test_dropout_border_of_the_threshold():
+    """p chosen so that the threshold is an element's own number (kept) and one above it (dropped): the lower 16 bits decide."""
+    n, seed, offset = 4096, 77, 3
+    r = ref.numbers(0, n, seed, offset)
+    x = torch.ones(n, device="cuda")
+    for e in (0, 1, 6, 7, 8, 1001, 4095):
+        for up in (0, 1):
+            p = (int(r[e]) + up) / 2 ** 32
+            y = dropout(x, p, seed, offset).cpu()
+            assert torch.equal(y != 0, ref.keep((n,), p, seed, offset))
+            assert bool(y[e] != 0) == (up == 0)
+
+
+@gpu
+def test_dropout_extremes():
+    x = torch.tensor([1.0, -2.0, float("inf"), float("-inf"), float("nan")] * 100, device="cuda")
+    assert torch.equal(dropout(x, 0.0, 5).nan_to_num(7.0), x.nan_to_num(7.0))
+    assert torch.equal(dropout(x, 2.0 ** -34, 5).nan_to_num(7.0), x.nan_to_num(7.0))       # rounds to zero
+    for p in (1.0, 1 - 2.0 ** -34):
+        assert torch.equal(dropout(x, p, 5), torch.zeros_like(x))                          # no inf * 0
+    m = ref.keep((500,), 0.5, 5, 0).cuda()
+    y = dropout(x, 0.5, 5)
+    assert torch.equal(y[~m], torch.zeros_like(y[~m])) and torch.equal(y[m].nan_to_num(7.0), (2 * x[m]).nan_to_num(7.0))
+    assert dropout(x[:0], 0.5, 5).shape == (0,)
+    assert dropout(torch.ones((), device="cuda"), 0.5, 1).shape == ()
+
+
+@gpu
+def test_dropout_seeds_and_layouts():
+    x = torch.randn(37, 19, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    want = dropout(x, 0.3, -5, 11)
+    assert torch.equal(want, dropout(x, 0.3, 2 ** 64 - 5, 11))
+    assert torch.equal(want, dropout(x, 0.3, torch.tensor([-5], device="cuda"), 11))
+    assert torch.equal(want, dropout(x, 0.3, torch.tensor(-5, device="cuda"), 11))
+    assert torch.equal(want, dropout(x.view(19, 37), 0.3, -5, 11).view(37, 19))            # the row-major index counts, not the shape
+    assert torch.equal(want, dropout(x.t().contiguous().t(), 0.3, -5, 11))                 # nor the strides
+    wide = torch.zeros(37, 40, device="cuda")
+    wide[:, 3:22] = x
+    assert torch.equal(want, dropout(wide[:, 3:22], 0.3, -5, 11))
+    flat = torch.zeros(37 * 19 + 1, device="cuda")
+    flat[1:] = x.reshape(-1)
+    assert torch.equal(want, dropout(flat[1:].view(37, 19), 0.3, -5, 11))                  # starts four bytes into an allocation
+    half = torch.zeros(37 * 19 + 1, device="cuda", dtype=F16)
+    half[1:] = x.reshape(-1)
+    assert torch.equal(dropout(half[1:], 0.3, -5, 11), dropout(x.half().reshape(-1), 0.3, -5, 11))
+    one = x[:1].expand(37, 19)
+    assert torch.equal(dropout(one, 0.3, -5, 11), dropout(one.contiguous(), 0.3, -5, 11))
+    for bad in (dict(p=1.5), dict(p=-0.1), dict(p=float("nan")), dict(seed=1 << 64), dict(seed=-(1 << 63) - 1), dict(offset=-1), dict(offset=1 << 64),
+                dict(seed=torch.zeros(2, device="cuda", dtype=torch.int64)), dict(seed=torch.zeros(1, device="cuda")), dict(seed=torch.zeros(1, dtype=torch.int64))):
+        with pytest.raises(hip.HipError):
+            dropout(x, **{**dict(p=0.5, seed=1), **bad})
+    with pytest.raises(TypeError):
+        dropout(x, 0.5, 1.5)
+    with pytest.raises(hip.HipError):
+        dropout(x.double(), 0.5, 1)
+
+
+@gpu
+def test_dropout_beyond_32_bit_indexes():
+    n = (1 << 32) + 4099
+    x = torch.ones(n, device="cuda", dtype=F16)
+    y = dropout(x, 0.25, 42, 7)
+    del x
+    for first in (0, (1 << 31) - 1000, (1 << 32) - 1000, n - 2000):
+        assert torch.equal((y[first:first + 2000] != 0).cpu(), ref.keep((2000,), 0.25, 42, 7, first=first))
+
+
+# ---------------------------------------------------------------------------------------------- layer_norm and the join
+
+TYPES = [(F32, None, F32), (F16, None, F32), (BF16, None, BF16), (F32, F32, F32), (F16, F16, F16), (BF16, BF16, F32), (F16, F32, F32), (BF16, F32, BF16)]
+SHAPES = [(1, 1), (5, 1), (3, 2), (1, 7), (4, 8), (130, 16), (67, 24), (33, 100), (9, 255), (700, 256), (41, 257), (19, 512), (13, 520), (7, 1021), (6, 1024),
+          (5, 1537), (4, 2048), (3, 2051), (5, 4096), (2, 5000), (3, 8192), (2, 16384), (3, 16391), (2, 40000)]
+
+
+@gpu
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(str(d)[6:] for d in t))
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_norm_against_float64(types, shape):
+    affine = ("both", "weight", "bias", "none")[(shape[0] + shape[1]) % 4]
+    check(operands(shape, *types, affine, seed=shape[0] * 1000 + shape[1]), p=0.1, seed=1234567 + shape[1], offset=3)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [0, 1, 2, 15, 16, 17, 255, 2047, 5000])
+@pytest.mark.parametrize("cols", [8, 72, 256, 1000])
+def test_norm_numbers_of_rows(rows, cols):
+    """Rows that fill no workgroup, exactly one, several; sums of the parameters' gradients over one row and many."""
+    check(operands((rows, cols), F32, F32, F32, "both", seed=rows + cols), p=0.2, seed=rows, offset=1)
+    check(operands((rows, cols), BF16, None, F32, "both", seed=rows + cols + 1))
+
+
+@gpu
+@pytest.mark.parametrize("affine", ["both", "weight", "bias", "none"])
+def test_norm_shapes_and_strides(affine):
+    g = torch.Generator("cuda").manual_seed(2)
+    base = torch.randn(6, 5, 300, device="cuda", generator=g)
+    for view in (base[:, :, 20:276], base[:, :, 3:260], base[:, :, :250], base[:, 2, 1:258], base.transpose(0, 1)[..., :256], base.permute(2, 1, 0)[:64],
+                 base[:1, :, 7:71].expand(4, 5, 64), base[3, 4, 10:266], base[::2, :, :128], base.flatten()[1:1 + 256 * 30].view(30, 256)):
+        o = operands(tuple(view.shape), F32, None, F32, affine, seed=4)
+        check(o, x_view=view)
+        o = operands(tuple(view.shape), F32, F32, F32, affine, seed=5)
+        wide = torch.randn(*view.shape[:-1], view.shape[-1] + 9, device="cuda", generator=g)
+        o["residual"] = wide[..., 4:4 + view.shape[-1]]
+        o["dy"] = o["dy"][..., :1].expand(view.shape)
+        check(o, p=0.5, seed=8, offset=9, x_view=view)
+
+
+@gpu
+def test_norm_half_precision_unaligned():
+    base = torch.randn(50 * 300 + 1, device="cuda", dtype=F16, generator=torch.Generator("cuda").manual_seed(3))
+    for start in (0, 1):
+        for cols in (256, 250):
+            view = base[start:start + 50 * 300].view(50, 300)[:, 1:1 + cols]
+            o = operands((50, cols), F16, F16, F16, "both", seed=6)
+            check(o, p=0.25, seed=3, x_view=view)
+
+
+@gpu
+def test_norm_rows_of_special_values():
+    """Constant rows, large offsets, and rows with infinities or NaN, which spoil their own results only."""
+    x = torch.randn(40, 256, device="cuda", generator=torch.Generator("cuda").manual_seed(4))
+    x[3] = 5.0
+    x[4] = 0.0
+    x[5] += 1000.0
+    x[6] *= 1e-20
+    x[7] *= 1e12
+    o = operands((40, 256), F32, None, F32, "both", seed=7)
+    want, grads = check({**o, "x": x})
+    assert torch.equal(layer_norm(x, o["weight"], o["bias"])[3:5], o["bias"].expand(2, 256))
+    clean = layer_norm(x, o["weight"], o["bias"])
+    x[10, 3], x[20, 100], x[30, 255] = float("inf"), float("nan"), float("-inf")
+    y = layer_norm(x, o["weight"], o["bias"])
+    bad = torch.zeros(40, dtype=torch.bool, device="cuda")
+    bad[[10, 20, 30]] = True
+    assert torch.equal(y[~bad], clean[~bad]) and bool(y[bad].isnan().all())
+    leaf = x.clone().requires_grad_()
+    dx, = torch.autograd.grad(layer_norm(leaf, o["weight"], o["bias"]), leaf, o["dy"])
+    assert torch.equal(dx[~bad], grads["x"][~bad]) and bool(dx[bad].isnan().all())
+
+
+@gpu
+def test_join_drops_non_finite_values():
+    x = torch.randn(16, 256, device="cuda", generator=torch.Generator("cuda").manual_seed(5))
+    m = ref.keep((16, 256), 0.5, 21, 2).cuda()
+    r = torch.randn(16, 256, device="cuda", generator=torch.Generator("cuda").manual_seed(6))
+    want = dropout_add_layer_norm(torch.where(m, x, torch.zeros(())).contiguous(), r, p=0.5, seed=21, offset=2)
+    spoiled = torch.where(m, x, torch.tensor([float("nan"), float("inf")], device="cuda").repeat(128))
+    assert torch.equal(dropout_add_layer_norm(spoiled, r, p=0.5, seed=21, offset=2), want)
+
+
+@gpu
+@pytest.mark.parametrize("types", [(F32, F32, F32), (BF16, BF16, F32), (F16, F32, F32)], ids=str)
+@pytest.mark.parametrize("cols", [256, 250, 257])
+def test_join_is_dropout_then_norm(types, cols):
+    """One mask for the separate calls and the join; p = 0 and p = 1; the seed as a tensor."""
+    o = operands((77, cols), *types, "both", seed=cols)
+    args = o["x"], o["residual"], o["weight"], o["bias"]
+    for p in (0.0, 0.3, 1.0):
+        factor = ref.keep((77, cols), p, 5, 6).double() * ref.scale(p)
+        assert torch.equal((dropout(torch.ones_like(o["x"]), p, 5, 6) != 0).cpu(), factor != 0)
+        want = ref.norm(o["x"], o["weight"], o["bias"], 1e-5, o["residual"], factor)
+        within(dropout_add_layer_norm(*args, p=p, seed=5, offset=6), want["y"], bounds(want, 1e-5, types[1], types[0], types[2])["y"], "y")
+    a = dropout_add_layer_norm(*args, p=0.3, seed=5, offset=6)
+    assert torch.equal(a, dropout_add_layer_norm(*args, p=0.3, seed=torch.tensor([5], device="cuda"), offset=6))
+
+
+@gpu
+def test_gradients_against_differences():
+    """Directional derivatives of the float64 forward pass; tolerance: the bounds of the gradients, summed along the direction."""
+    o = operands((23, 40), F32, F32, F32, "both", seed=11)
+    p, seed, offset = 0.25, 31, 4
+    want, grads = check(o, p=p, seed=seed, offset=offset)
+    factor = ref.keep((23, 40), p, seed, offset).double() * ref.scale(p)
+    tol = bounds(want, 1e-5, F32, F32, F32, ref.scale(p))
+    g = torch.Generator().manual_seed(12)
+    t = {k: o[k].double().cpu() for k in ("x", "residual", "weight", "bias")}
+    loss = lambda t: float((ref.norm(t["x"], t["weight"], t["bias"], 1e-5, t["residual"], factor)["y"] * want["dy"]).sum())     # noqa: E731
+    for k in t:
+        v, h = torch.randn(t[k].shape, generator=g, dtype=torch.float64), 1e-6
+        slope = (loss({**t, k: t[k] + h * v}) - loss({**t, k: t[k] - h * v})) / (2 * h)
+        assert abs(slope - float((grads[k].double().cpu() * v).sum())) <= float((tol["d" + k] * v.abs()).sum()) + 1e-6
+
+
+@gpu
+def test_only_the_wanted_gradients():
+    o = operands((30, 256), F32, F32, F32, "both", seed=13)
+    names = ("x", "residual", "weight", "bias")
+    full = None
+    for wanted in (names, ("x",), ("residual",), ("weight",), ("bias",), ("x", "bias"), ("residual", "weight")):
+        t = {k: o[k].detach().clone().requires_grad_(k in wanted) for k in names}
+        y = dropout_add_layer_norm(*t.values(), p=0.1, seed=3, offset=1)
+        y.backward(o["dy"])
+        got = {k: t[k].grad for k in names}
+        full = full or got
+        for k in names:
+            assert got[k] is None if k not in wanted else torch.equal(got[k], full[k])
+    with torch.no_grad():
+        assert not dropout_add_layer_norm(*t.values(), p=0.1, seed=3, offset=1).requires_grad
+
+
+@gpu
+def test_second_derivatives():
+    """dropout is linear: its gradient's graph is its own; the normalisations refuse to build one."""
+    x = torch.randn(4, 40, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).requires_grad_()
+    y = dropout(x, 0.5, 6) ** 2
+    g, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    second, = torch.autograd.grad(g.sum(), x)
+    assert torch.equal(second.cpu(), ref.keep((4, 40), 0.5, 6, 0).float() * 8)
+    for y in (layer_norm(x), dropout_add_layer_norm(x, x, p=0.5, seed=6)):
+        with pytest.raises(hip.HipError, match="not differentiable"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+@gpu
+def test_same_call_same_bits():
+    o = operands((3000, 257), BF16, F32, F32, "both", seed=14)
+    runs = []
+    for _ in range(3):
+        t = [o[k].detach().requires_grad_() for k in ("x", "residual", "weight", "bias")]
+        y = dropout_add_layer_norm(*t, p=0.1, seed=3, offset=1)
+        runs.append([y.detach(), *torch.autograd.grad(y, t, o["dy"])])
+    for other in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
+@gpu
+def test_shared_weight_and_broadcast_inputs():
+    """One weight used by two calls, a residual broadcast over rows: autograd adds the gradients up."""
+    o = operands((12, 64), F32, F32, F32, "both", seed=15)
+    w, b, row = o["weight"].requires_grad_(), o["bias"].requires_grad_(), o["residual"][:1].detach().clone().requires_grad_()
+    y = layer_norm(dropout_add_layer_norm(o["x"], row.expand(12, 64), w, b, p=0.2, seed=1, offset=1), w, b)
+    y.backward(o["dy"])
+    factor = ref.keep((12, 64), 0.2, 1, 1).double() * ref.scale(0.2)
+    first = ref.norm(o["x"], w, b, 1e-5, row.expand(12, 64), factor)
+    second = ref.norm(first["y"], w, b, 1e-5, dy=o["dy"])
+    first = ref.norm(o["x"], w, b, 1e-5, row.expand(12, 64), factor, second["dx"])
+    # two chained operators, each off by less than 2^-24 * 100 of its results' size (D = 64)
+    for got, want in ((w.grad, first["dweight"] + second["dweight"]), (b.grad, first["dbias"] + second["dbias"]), (row.grad, first["dresidual"].sum(0, keepdim=True))):
+        assert float((got.double().cpu() - want).norm() / want.norm()) < 200 * E32
+
+
+@gpu
+def test_refusals():
+    x = torch.zeros(4, 16, device="cuda")
+    w = torch.ones(16, device="cuda")
+    for call in (lambda: layer_norm(x.double()), lambda: layer_norm(x, w[:8]), lambda: layer_norm(x, w.half()), lambda: layer_norm(x.half(), w, w.half()),
+                 lambda: layer_norm(x, w.cpu()), lambda: layer_norm(torch.ones((), device="cuda")), lambda: layer_norm(x[:, :0]), lambda: layer_norm(x, eps=0.0),
+                 lambda: layer_norm(x, eps=-1.0), lambda: layer_norm(x, eps=float("nan")), lambda: dropout_add_layer_norm(x, x[:1]),
+                 lambda: dropout_add_layer_norm(x, x.half()), lambda: dropout_add_layer_norm(x.half(), x.bfloat16()), lambda: dropout_add_layer_norm(x, x.cpu()),
+                 lambda: dropout_add_layer_norm(x, x, p=1.1), lambda: dropout_add_layer_norm(x, x, p=0.1, offset=-1)):
+        with pytest.raises(hip.HipError):
+            call()
+    y, mean, rstd = hip.norm_forward(x, w, w, want_stats=True)
+    for bad in (dict(dy=y.half()), dict(dy=y[:2]), dict(mean=mean[:2]), dict(rstd=rstd.double())):
+        with pytest.raises(hip.HipError):
+            hip.norm_backward(**{**dict(dy=y, x=x, mean=mean, rstd=rstd, weight=w), **bad})
+
+
+@gpu
+def test_inputs_changed_between_the_passes_are_noticed():
+    x, seed = torch.randn(8, 32, device="cuda").requires_grad_(), torch.tensor([4], device="cuda")
+    y = dropout(x, 0.5, seed)
+    seed += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+@gpu
+def test_on_another_stream():
+    side = torch.cuda.Stream()
+    o = operands((500, 256), F32, F32, F32, "both", seed=16)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        want, grads = check(o, p=0.1, seed=2)
+    side.synchronize()
+
+
+@gpu
+def test_captured_step_draws_new_masks():
+    """Forward and backward of both operators in one graph, the seed advanced inside it; every replay against eager calls, with eager
+    work between the replays."""
+    o = operands((300, 256), BF16, BF16, F32, "both", seed=17)
+    seed = torch.tensor([100], device="cuda")
+    keep = {}
+
+    def step(seed):
+        h = hip.dropout(o["x"], 0.2, seed, 1)
+        y, mean, rstd = hip.norm_forward(h, o["weight"], o["bias"], 1e-5, o["residual"], 0.3, seed, 2, want_stats=True)
+        dh, dres, dw, db = hip.norm_backward(o["dy"], h, mean, rstd, o["weight"], o["bias"], 1e-5, o["residual"], 0.3, seed, 2)
+        return y, hip.dropout(dh, 0.2, seed, 1), dres, dw, db
+
+    step(seed)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        seed += 1
+        keep["out"] = step(seed)
+    for n in range(1, 5):
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in keep["out"]]
+        want = step(100 + n)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), n
+        torch.randn(1000, device="cuda").sum().item()
+
+
+@gpu
+def test_captured_autograd_step():
+    """The same through autograd, captured with leaves of its own."""
+    o = operands((64, 128), F32, F32, F32, "both", seed=18)
+    seed = torch.tensor([7], device="cuda")
+    leaves = [o[k].detach().clone().requires_grad_() for k in ("x", "residual", "weight", "bias")]
+    eager = [t.detach().clone().requires_grad_() for t in leaves]
+
+    def step(t, seed):
+        y = dropout_add_layer_norm(*t, p=0.4, seed=seed, offset=5)
+        return [y.detach(), *torch.autograd.grad(y, t, o["dy"])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(leaves, seed)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(leaves, seed)
+    for n in range(3):
+        seed.fill_(50 + n)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step(eager, 50 + n))), n
+
+
+@gpu
+def test_block_of_the_tracker_trains():
+    """A feed-forward block as the tracker has it -- norm(x + dropout(attn)), norm2(x + dropout(linear(dropout(gelu(linear(x)))))) -- with all
+    gradients, against float64 autograd with the same masks.  The products run in float64 here, so what is off is the operators' own:
+    six of them, each below 2^-24 * 150 of its result's norm (D = 1024 at most), chained through factors near one."""
+    g = torch.Generator().manual_seed(19)
+    R, D, H, p, seed = 96, 256, 1024, 0.1, 2024
+    t = {k: torch.randn(*s, generator=g) * c for k, s, c in (("x", (R, D), 1), ("attn", (R, D), 1), ("w1", (H, D), D ** -0.5), ("w2", (D, H), H ** -0.5),
+                                                              ("n1", (D,), 1), ("b1", (D,), 1), ("n2", (D,), 1), ("b2", (D,), 1))}
+    dy = torch.randn(R, D, generator=g)
+    a = {k: v.cuda().requires_grad_() for k, v in t.items()}
+    lin = lambda x, w: (x.double() @ w.double().t()).float()     # noqa: E731
+    h = dropout_add_layer_norm(a["attn"], a["x"], a["n1"], a["b1"], p=p, seed=seed, offset=0)
+    f = lin(dropout(torch.nn.functional.gelu(lin(h, a["w1"]).double()).float(), p, seed, 1), a["w2"])
+    y = layer_norm(dropout(f, p, seed, 2) + h, a["n2"], a["b2"])
+    y2 = dropout_add_layer_norm(f, h, a["n2"], a["b2"], p=p, seed=seed, offset=2)
+    y2.backward(dy.cuda())
+    b = {k: v.double().requires_grad_() for k, v in t.items()}
+    fac = [ref.keep(s, p, seed, k).double() * ref.scale(p) for k, s in enumerate(((R, D), (R, H), (R, D)))]
+    ln = lambda z, w, c: torch.nn.functional.layer_norm(z, (D,), w, c, 1e-5)     # noqa: E731
+    h64 = ln(b["x"] + b["attn"] * fac[0], b["n1"], b["b1"])
+    f64 = (torch.nn.functional.gelu(h64 @ b["w1"].t()) * fac[1]) @ b["w2"].t()
+    y64 = ln(h64 + f64 * fac[2], b["n2"], b["b2"])
+    y64.backward(dy.double())
+    off = lambda got, want: float((got.detach().double().cpu() - want.detach()).norm() / want.detach().norm())     # noqa: E731
+    assert off(y, y64) < 1000 * E32 and off(y2, y64) < 1000 * E32
+    for k in t:
+        assert off(a[k].grad, b[k].grad) < 1000 * E32, (k, off(a[k].grad, b[k].grad))
