@@ -5,29 +5,9 @@
 //   dw = sum over rows of dy xhat;  db = sum over rows of dy
 // All sums are fp32.  z is rebuilt from x, residual and the mask in the backward pass: storing it would move the same bytes (one write
 // and one read against two reads for one), round it, and hold one more tensor.
-#include "train.hpp"
+#include "norm.hpp"
 
 namespace lbm {
-
-// the eight z values of a chunk, and the mask bits when something is dropped
-template <class TX, class TR, int RES>
-__device__ __forceinline__ uint32_t load_z(const NormArgs& a, const DropKey& key, long long row, long long c, int nv, float (&z)[8]) {
-  Vec8<TX> vx;
-  vx.load(reinterpret_cast<const TX*>(a.x) + row * a.ld_x + c, nv);
-  uint32_t m = 0xffu;
-  Vec8<TR> vr;
-  float scale = 1.0f;
-  if (RES) {
-    vr.load(reinterpret_cast<const TR*>(a.residual) + row * a.ld_r + c, nv);
-    if (a.drop.on) {
-      m = keep8((uint64_t)(row * a.cols + c), key, a.drop.tm1);
-      scale = a.drop.scale;
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) z[j] = join_one<RES>(vx.get(j), RES ? vr.get(j) : 0.0f, m >> j & 1, scale);
-  return m;
-}
 
 template <class TX, class TR, int RES>
 __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
@@ -144,34 +124,12 @@ __global__ __launch_bounds__(256) void norm_wide_dw_kernel(NormArgs a) {
   }
 }
 
-// dweight / dbias = the partial sums added up in a fixed order; 16 columns x 16 slices of the partials a workgroup
-template <class T>
-__global__ __launch_bounds__(256) void norm_dw_finish_kernel(const float* part, int parts, long long cols, T* dweight, T* dbias) {
-  __shared__ float sm[16][17];
-  const int tc = threadIdx.x & 15, tg = threadIdx.x >> 4;
-  const long long c = (long long)blockIdx.x * 16 + tc;              // over 2 cols: dweight, then dbias
-  float s = 0.0f;
-  if (c < 2 * cols)
-    for (int g = tg; g < parts; g += 16) s += part[(long long)g * 2 * cols + c];
-  sm[tg][tc] = s;
-  __syncthreads();
-  if (tg == 0 && c < 2 * cols) {
-    s = 0.0f;
-#pragma unroll
-    for (int g = 0; g < 16; ++g) s += sm[g][tc];
-    T* o = c < cols ? dweight : dbias;
-    if (o != nullptr) o[c < cols ? c : c - cols] = (T)s;
-  }
-}
-
-static int wide_parts(long long rows, long long cols) {
+int norm_wide_parts(long long rows, long long cols) {
   const long long slabs = (cols + 2047) / 2048;                     // workgroups along the columns; fill ~1024 with rows
   long long g = (1024 + slabs - 1) / slabs;
   if (g > rows) g = rows;
   return (int)(g < 1 ? 1 : g);
 }
-
-uint64_t norm_workspace_bytes(long long rows, long long cols) { return (uint64_t)wide_parts(rows, cols) * 2 * (uint64_t)cols * sizeof(float); }
 
 template <class TX, class TR, int RES> static int wide_forward(const NormArgs& a, hipStream_t s) {
   const unsigned grid = (unsigned)(a.rows < (1ll << 30) ? a.rows : (1ll << 30));
@@ -185,42 +143,15 @@ template <class TX, class TR, int RES> static int wide_backward(const NormArgs& 
     if (check_launch("norm_backward")) return -1;
   }
   if (a.dweight != nullptr || a.dbias != nullptr) {
-    const int parts = wide_parts(a.rows, a.cols);
+    const int parts = norm_wide_parts(a.rows, a.cols);
     norm_wide_dw_kernel<TX, TR, RES><<<dim3((unsigned)((a.cols + 2047) / 2048), parts), 256, 0, s>>>(a);
     if (check_launch("norm_backward")) return -1;
-    const unsigned fin = (unsigned)((2 * a.cols + 15) / 16);
-    if (a.p_f32)
-      norm_dw_finish_kernel<float><<<fin, 256, 0, s>>>(a.workspace, parts, a.cols, (float*)a.dweight, (float*)a.dbias);
-    else
-      norm_dw_finish_kernel<TX><<<fin, 256, 0, s>>>(a.workspace, parts, a.cols, (TX*)a.dweight, (TX*)a.dbias);
-    return check_launch("norm_backward");
+    return norm_finish(a, parts, s);
   }
   return 0;
 }
 
-// calls f<TX, TR, RES>(a, s) for the types of a
-#define NORM_DISPATCH(F, a, s)                                                                            \
-  do {                                                                                                    \
-    if (a.residual == nullptr) {                                                                          \
-      if (a.x_type == kF32) return F<float, float, 0>(a, s);                                              \
-      if (a.x_type == kF16) return F<_Float16, _Float16, 0>(a, s);                                        \
-      return F<__bf16, __bf16, 0>(a, s);                                                                  \
-    }                                                                                                     \
-    if (a.x_type == kF32) return F<float, float, 1>(a, s);                                                \
-    if (a.x_type == kF16) return a.y_type == kF32 ? F<_Float16, float, 1>(a, s) : F<_Float16, _Float16, 1>(a, s); \
-    return a.y_type == kF32 ? F<__bf16, float, 1>(a, s) : F<__bf16, __bf16, 1>(a, s);                     \
-  } while (0)
-
-int norm_forward(const NormArgs& a, hipStream_t stream) {
-  if (a.rows == 0) return 0;
-  ProfScope prof("norm_forward", stream, 8.0 * a.rows * a.cols,
-                 (double)a.rows * a.cols * (elem_size(a.x_type) + elem_size(a.y_type) * (a.residual ? 2.0 : 1.0)));
-  NORM_DISPATCH(wide_forward, a, stream);
-}
-int norm_backward(const NormArgs& a, hipStream_t stream) {
-  ProfScope prof("norm_backward", stream, 14.0 * a.rows * a.cols,
-                 (double)a.rows * a.cols * (2.0 * elem_size(a.x_type) + elem_size(a.y_type) * (a.residual ? 3.0 : 1.0)));
-  NORM_DISPATCH(wide_backward, a, stream);
-}
+int norm_wide_forward(const NormArgs& a, hipStream_t stream) { NORM_DISPATCH(wide_forward, a, stream); }
+int norm_wide_backward(const NormArgs& a, hipStream_t stream) { NORM_DISPATCH(wide_backward, a, stream); }
 
 }  // namespace lbm
