@@ -98,7 +98,7 @@ int lbm_hip_dropout(const void* x, void* y, int64_t n, int32_t type, double p, u
  * rstd = 1 / sqrt(mean((z - mean)^2) + eps).  Statistics and sums are fp32.  Types: x and dx x_type; residual, y, dy and dresidual
  * res_type (= x_type, or LBM_TYPE_F32: half-precision products beside an fp32 residual stream; without a residual = x_type);
  * weight, bias and their gradients param_type (= x_type or LBM_TYPE_F32), either may be NULL.  Element strides between rows:
- * ld_x, ld_residual, ld_dy (>= cols); outputs are dense.  1 <= cols <= 2^28.
+ * ld_x, ld_residual, ld_dy (>= cols, < 2^31); outputs are dense and overlap no input.  1 <= cols <= 2^28.
  *
  * forward: reads x, residual, weight, bias; writes y, and mean / rstd (fp32 [rows], both or neither).
  * backward: reads dy, x, residual, weight, mean, rstd; writes the non-NULL ones of dx, dresidual, dweight, dbias

@@ -757,6 +757,7 @@ static int norm_args(const char* what, const lbm_hip_norm_desc* d, NormArgs& a) 
   LBM_REQUIRE(d->param_type == d->x_type || d->param_type == LBM_TYPE_F32, "%s: param_type must be x_type or fp32", what);
   LBM_REQUIRE(d->rows == 0 || d->x != nullptr, "%s: null x", what);
   LBM_REQUIRE(d->ld_x >= d->cols && (d->residual == nullptr || d->ld_residual >= d->cols), "%s: a row stride is shorter than a row", what);
+  LBM_REQUIRE(d->ld_x < (1ll << 31) && (d->residual == nullptr || d->ld_residual < (1ll << 31)), "%s: a row stride of 2^31 elements or more", what);
   LBM_REQUIRE(d->eps >= 1.17549435e-38f && d->eps <= 3.402823466e38f, "%s: eps must be a positive normal fp32 number", what);
   LBM_REQUIRE(joined || d->p == 0.0, "%s: dropout needs a residual to be added to", what);
   if (make_drop(d->p, d->seed, d->seed_dev, d->offset, a.drop)) return -1;
@@ -797,7 +798,7 @@ int lbm_hip_norm_backward(const lbm_hip_norm_desc* d, lbm_stream_t stream) {
   NormArgs a;
   if (norm_args("norm_backward", d, a)) return -1;
   LBM_REQUIRE(a.rows == 0 || (a.dy != nullptr && a.mean != nullptr && a.rstd != nullptr), "norm_backward: null dy, mean or rstd");
-  LBM_REQUIRE(d->ld_dy >= d->cols, "norm_backward: a row stride is shorter than a row");
+  LBM_REQUIRE(d->ld_dy >= d->cols && d->ld_dy < (1ll << 31), "norm_backward: a row stride is shorter than a row, or 2^31 elements or more");
   LBM_REQUIRE(a.dresidual == nullptr || a.residual != nullptr, "norm_backward: dresidual without a residual");
   if (a.dweight != nullptr || a.dbias != nullptr) {
     LBM_REQUIRE(a.workspace != nullptr && ((uintptr_t)a.workspace & 15) == 0 && a.workspace_bytes >= norm_workspace_bytes(a.rows, a.cols),

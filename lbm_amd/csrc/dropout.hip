@@ -19,17 +19,21 @@ int make_drop(double p, uint64_t seed, const void* seed_ptr, uint64_t offset, Dr
 template <class T>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* x, T* y, long long n, DropArgs d) {
   const DropKey key = drop_key(d);
+  const uint32_t limit = keep_limit(d.tm1);
   const long long chunks = (n + 7) >> 3, step = (long long)gridDim.x * 256;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < chunks; i += step) {
     const long long left = n - 8 * i;
     const int nv = left < 8 ? (int)left : 8;
     Vec8<T> v;
-    v.load(x + 8 * i, nv);
-    const uint32_t m = block_keep((uint64_t)i, key, d.tm1);
-    float f[8];
+    if (nv == 8) v.load(x + 8 * i);
+    else v.load_some(x + 8 * i, nv);
+    if (d.on) {
+      const Keep8 m = block_keep((uint64_t)i, key, d.tm1);
+      float f[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = (m >> j & 1) ? v.get(j) * d.scale : 0.0f;
-    v.set(f);
+      for (int j = 0; j < 8; ++j) f[j] = m.kept(j, limit) ? v.get(j) * d.scale : 0.0f;
+      v.set(f);
+    }
     v.store(y + 8 * i, nv);
   }
 }

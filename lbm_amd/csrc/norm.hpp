@@ -4,39 +4,21 @@
 
 namespace lbm {
 
-constexpr long long kNormRowMax = 16384;      // longest row that a workgroup holds in registers; beyond: norm_wide.hip
+// rows that a team holds in registers; shorter (no eight elements to read at once) and longer ones: norm_wide.hip
+constexpr long long kNormRowMin = 8, kNormRowMax = 16384;
 
 int norm_wide_forward(const NormArgs& a, hipStream_t stream);
 int norm_wide_backward(const NormArgs& a, hipStream_t stream);
 int norm_wide_parts(long long rows, long long cols);
 int norm_finish(const NormArgs& a, int parts, hipStream_t stream);     // workspace [parts][2][cols] -> dweight, dbias
 
-// the eight z values of a chunk, and the mask bits when something is dropped
-template <class TX, class TR, int RES>
-__device__ __forceinline__ uint32_t load_z(const NormArgs& a, const DropKey& key, long long row, long long c, int nv, float (&z)[8]) {
-  Vec8<TX> vx;
-  vx.load(reinterpret_cast<const TX*>(a.x) + row * a.ld_x + c, nv);
-  uint32_t m = 0xffu;
-  Vec8<TR> vr;
-  float scale = 1.0f;
-  if (RES) {
-    vr.load(reinterpret_cast<const TR*>(a.residual) + row * a.ld_r + c, nv);
-    if (a.drop.on) {
-      m = keep8((uint64_t)(row * a.cols + c), key, a.drop.tm1);
-      scale = a.drop.scale;
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) z[j] = join_one<RES>(vx.get(j), RES ? vr.get(j) : 0.0f, m >> j & 1, scale);
-  return m;
-}
-
 // ---- teams: the threads that share a row ------------------------------------------------------------------------------
-// Thread tl of a team of T holds the 8-element chunks tl, T + tl, ... (K of them) of its row in registers.  Up to 512 columns a team is a
-// power of two of lanes (a wave works on several short rows), up to 2048 a wave with K = 2 or 4 chunks a lane, beyond a workgroup.
+// Thread tl of a team of T threads holds the 8-element chunks tl, T + tl, ... (K of them) of its row in registers.  Rows up to 2048
+// columns belong to a power of two of lanes of one wave with K <= 4: of the pairs (T, K) that hold the row the one with the fewest
+// T * K chunks (a lane past the row's end costs as much as one inside), the larger T among equals.  Longer rows belong to a workgroup.
 struct NormShape {
   int k;            // chunks a thread
-  int shift;        // log2 of the lanes of a team (wave teams)
+  int shift;        // log2 of the lanes of a team (rows of a wave)
   int threads;      // of a workgroup
   bool block;       // a team is a workgroup
   int teams() const { return block ? 1 : threads >> shift; }
@@ -44,15 +26,56 @@ struct NormShape {
 inline NormShape norm_shape(long long cols) {
   NormShape s{1, 0, 256, false};
   const int chunks = (int)((cols + 7) / 8);
-  if (cols <= 2048) {
-    while (s.shift < 6 && (1 << s.shift) < chunks) ++s.shift;
-    s.k = chunks <= 64 ? 1 : chunks <= 128 ? 2 : 4;
-  } else {
+  if (chunks > 256) {
     s.block = true;
     s.k = 2;
     s.threads = (chunks + 127) / 128 * 64;
+    return s;
+  }
+  int best = 1 << 30;
+  for (int shift = 6; shift >= 0; --shift) {
+    const int k = (chunks + (1 << shift) - 1) >> shift;
+    if (k <= 4 && (k << shift) < best) {
+      best = k << shift;
+      s.k = k;
+      s.shift = shift;
+    }
   }
   return s;
+}
+
+// Where a chunk's eight elements are read: the last one of a row that is no multiple of eight is read from eight before the row's end on
+// and cut, so no load lies outside of the row and none waits for a branch.  cut = 8: the chunk lies past the row's end.
+struct Span {
+  int at, cut;
+  __device__ __forceinline__ Span() {}
+  __device__ __forceinline__ Span(int c, int cols) : at(min(c, cols - 8)), cut(min(c - at, 8)) {}
+};
+template <class TX> __device__ __forceinline__ void load_param(const void* p, int p_f32, const Span& s, float dflt, float (&v)[8]) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = dflt;
+  } else if (p_f32) {
+    Vec8<float> r;
+    r.load(reinterpret_cast<const float*>(p) + s.at);
+    r.cut(s.cut);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = r.get(j);
+  } else {
+    Vec8<TX> r;
+    r.load(reinterpret_cast<const TX*>(p) + s.at);
+    r.cut(s.cut);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = r.get(j);
+  }
+}
+// element offset of row r (below 2^32) at a stride below 2^31: one multiply
+__device__ __forceinline__ uint64_t row_at(uint32_t r, uint32_t ld, int c) { return (uint64_t)r * ld + (uint32_t)c; }
+// 1 / sqrt(v): v_rsq_f32 (1 ulp) and a Newton step in place of the correctly rounded square root and division (~25 instructions a row)
+__device__ __forceinline__ float rsqrt_newton(float v) {
+  const float r = __builtin_amdgcn_rsqf(v);
+  const float e = fmaf(-v * r, r, 1.0f);
+  return fmaf(0.5f * r, e, r);
 }
 
 __device__ __forceinline__ float lane16_sum(float v) {     // v + the value 16 lanes away (lane ^ 16)

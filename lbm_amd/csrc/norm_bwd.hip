@@ -8,11 +8,8 @@
 
 namespace lbm {
 
-#ifndef NB_U1
-#define NB_U1 2
-#define NB_U2 1
-#define NB_G 1024
-#define NB_GB 512
+#ifndef NB_G
+#define NB_G 512
 #endif
 
 // dweight / dbias from the first partial sum when it is the only one
@@ -26,154 +23,222 @@ template <class TX> __device__ __forceinline__ void put_part(const NormArgs& a, 
   else put_sum<TX>(a, which, c, v);
 }
 
-template <class TX, class TR, int RES, int K, int U, bool BLK>
-__global__ __launch_bounds__(BLK ? 1024 : 256) void norm_bwd_kernel(NormArgs a, int shift) {
-  __shared__ float red[BLK ? 64 : 4 * 512 * K];          // BLK: the row sums of two rows in turn; else: one sum of every wave, then of the other
-  const int lanes = BLK ? blockDim.x : K > 1 ? 64 : 1 << shift;
-  const int tl = BLK ? threadIdx.x : threadIdx.x & (lanes - 1);
-  const int team = BLK ? 0 : K > 1 ? threadIdx.x >> 6 : threadIdx.x >> shift;
-  const int teams = BLK ? 1 : K > 1 ? 4 : 256 >> shift;
-  const int cols = (int)a.cols;
+template <class TX, class TR, int K> struct BwdRow {
+  Vec8<TR> d[K];
+  Vec8<TX> x[K];
+  Vec8<TR> r[K];
+  float mean, rstd;
+};
+
+// One row of a team: xhat and g = dy w from what was loaded, their two sums (s1 = sum g, s2 = sum g xhat), the columns' sums.
+// w: this thread's weights, from LDS where K > 1 (their registers would cost a wave a SIMD; a fetch is two ds_read_b128 a chunk).
+// gone: a row past the last one, of which nothing counts.
+template <class TX, class TR, int RES, int K>
+__device__ __forceinline__ void bwd_row(const NormArgs& a, const DropKey& key, BwdRow<TX, TR, K>& in, const Span (&sp)[K], bool gone, long long row,
+                                        int lanes, int tl, const float* w, float (&xh)[K][8], float (&g)[K][8], Keep8 (&m)[K],
+                                        float (&dw)[K][8], float (&db)[K][8], float& s1, float& s2) {
+  s1 = s2 = 0.0f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    in.x[k].cut(sp[k].cut);
+    in.d[k].cut(gone ? 8 : sp[k].cut);
+    if (RES) in.r[k].cut(sp[k].cut);
+    if (RES && a.drop.on) {
+      m[k] = keep8((uint64_t)(row * a.cols + (k * lanes + tl) * 8), key, a.drop.tm1);
+      const uint32_t limit = keep_limit(a.drop.tm1);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) xh[k][j] = join_one<RES>(in.x[k].get(j), in.r[k].get(j), m[k].kept(j, limit), a.drop.scale);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) xh[k][j] = join_one<RES>(in.x[k].get(j), RES ? in.r[k].get(j) : 0.0f, true, 1.0f);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) xh[k][j] = (xh[k][j] - in.mean) * in.rstd;
+    if (gone || sp[k].cut != 0) {          // dy is zero there, but zero times an overflowed xhat is not
+#pragma unroll
+      for (int j = 0; j < 8; ++j) xh[k][j] = !gone && j < 8 - sp[k].cut ? xh[k][j] : 0.0f;
+    }
+    int at = (k * lanes + tl) * 8;
+    if (K > 1) asm volatile("" : "+v"(at));  // fetch the weights again for every row: kept across rows they take 8 K registers
+    const float* wk = K > 1 ? w + at : w;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float d = in.d[k].get(j);
+      g[k][j] = d * wk[j];
+      s1 += g[k][j];
+      s2 = fmaf(g[k][j], xh[k][j], s2);
+      dw[k][j] = fmaf(d, xh[k][j], dw[k][j]);
+      db[k][j] += d;
+    }
+  }
+}
+template <class TX, class TR, int RES, int K>
+__device__ __forceinline__ void bwd_put(const NormArgs& a, const Span (&sp)[K], long long at, int lanes, int tl, float c1, float c2, float rstd,
+                                        const float (&xh)[K][8], const float (&g)[K][8], const Keep8 (&m)[K]) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (sp[k].cut == 8) continue;
+    float dz[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dz[j] = rstd * (fmaf(-xh[k][j], c2, g[k][j] - c1));
+    const long long o = at + (k * lanes + tl) * 8;
+    if (RES && a.dresidual != nullptr) {
+      Vec8<TR> v;
+      v.set(dz);
+      v.store(reinterpret_cast<TR*>(a.dresidual) + o, 8 - sp[k].cut);
+    }
+    if (a.dx != nullptr) {
+      if (RES && a.drop.on) {
+        const uint32_t limit = keep_limit(a.drop.tm1);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dz[j] = m[k].kept(j, limit) ? dz[j] * a.drop.scale : 0.0f;
+      }
+      Vec8<TX> v;
+      v.set(dz);
+      v.store(reinterpret_cast<TX*>(a.dx) + o, 8 - sp[k].cut);
+    }
+  }
+}
+
+// Rows of lanes of a wave.  The next row's loads are issued when this row has become xhat and g, and pass behind its sums and stores.
+template <class TX, class TR, int RES, int K>
+__global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a, int shift) {
+  __shared__ __align__(16) float red[4 * 512 * K];         // the weights (K > 1); at the end one column sum of every wave
+  const int lanes = 1 << shift, tl = threadIdx.x & (lanes - 1), team = threadIdx.x >> shift, teams = 256 >> shift, cols = (int)a.cols;
   const float inv = 1.0f / (float)cols;
   DropKey key{};
   if (RES) key = drop_key(a.drop);
-  int nv[K];
-  float w[K][8], dw[K][8] = {}, db[K][8] = {};
+  Span sp[K];
+  float w[8], dw[K][8] = {}, db[K][8] = {};
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    nv[k] = min(8, cols - (k * lanes + tl) * 8);
-    load_param<TX>(a.weight, a.p_f32, (k * lanes + tl) * 8, nv[k], 1.0f, w[k]);
+    sp[k] = Span((k * lanes + tl) * 8, cols);
+    if (K == 1 || (int)threadIdx.x < lanes) load_param<TX>(a.weight, a.p_f32, sp[k], 1.0f, w);
+    if (K > 1 && (int)threadIdx.x < lanes) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) red[(k * lanes + tl) * 8 + j] = w[j];
+    }
   }
-  int par = 0;
-  for (long long base = (long long)blockIdx.x * (teams * U); base < a.rows; base += (long long)gridDim.x * (teams * U)) {
-    Vec8<TX> vx[U][K];
-    Vec8<TR> vr[U][K], vd[U][K];
-    float mean[U], rstd[U];
+  if (K > 1) __syncthreads();
+  BwdRow<TX, TR, K> in;
+  const auto load = [&](long long base) {                  // a team's row of the rows base .. base + teams - 1 (past the last: the last)
+    const uint32_t r = min((long long)team, a.rows - base - 1);
+    const TX* px = reinterpret_cast<const TX*>(a.x) + base * a.ld_x;
+    const TR* pr = reinterpret_cast<const TR*>(a.residual) + base * a.ld_r;
+    const TR* pd = reinterpret_cast<const TR*>(a.dy) + base * a.ld_dy;
+    in.mean = a.mean[base + r];
+    in.rstd = a.rstd[base + r];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long long row = base + u * teams + team;
-      const bool in = row < a.rows;
-      mean[u] = in ? a.mean[row] : 0.0f;
-      rstd[u] = in ? a.rstd[row] : 0.0f;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {       // past the row's end, and past the last row: zeros
-        const int c = (k * lanes + tl) * 8, n = in ? nv[k] : 0;
-        vd[u][k].load(reinterpret_cast<const TR*>(a.dy) + row * a.ld_dy + c, n);
-        vx[u][k].load(reinterpret_cast<const TX*>(a.x) + row * a.ld_x + c, n);
-        if (RES) vr[u][k].load(reinterpret_cast<const TR*>(a.residual) + row * a.ld_r + c, n);
-      }
+    for (int k = 0; k < K; ++k) {
+      in.d[k].load(pd + row_at(r, (uint32_t)a.ld_dy, sp[k].at));
+      in.x[k].load(px + row_at(r, (uint32_t)a.ld_x, sp[k].at));
+      if (RES) in.r[k].load(pr + row_at(r, (uint32_t)a.ld_r, sp[k].at));
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long long row = base + u * teams + team;
-      float xh[K][8], s1 = 0.0f, s2 = 0.0f;
-      uint32_t m[K];
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        m[k] = 0xffu;
-        float scale = 1.0f;
-        if (RES && a.drop.on) {
-          m[k] = keep8((uint64_t)(row * a.cols + (k * lanes + tl) * 8), key, a.drop.tm1);
-          scale = a.drop.scale;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float z = join_one<RES>(vx[u][k].get(j), RES ? vr[u][k].get(j) : 0.0f, m[k] >> j & 1, scale);
-          xh[k][j] = (z - mean[u]) * rstd[u];
-        }
-        if (nv[k] < 8) {                  // nothing past the row's end may reach a sum (0 times an overflowed mean * rstd is no zero)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) xh[k][j] = j < nv[k] ? xh[k][j] : 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float d = vd[u][k].get(j), g = d * w[k][j];
-          s1 += g;
-          s2 = fmaf(g, xh[k][j], s2);
-          dw[k][j] = fmaf(d, xh[k][j], dw[k][j]);
-          db[k][j] += d;
-        }
-      }
-      if (BLK) {
-        // one barrier a row: the next row writes the other half, and the one after it finds every thread past this row's reads
-        s1 = wave64_sum(s1);
-        s2 = wave64_sum(s2);
-        float* sm = red + 32 * par;
-        par ^= 1;
-        if ((threadIdx.x & 63) == 0) {
-          sm[2 * (threadIdx.x >> 6)] = s1;
-          sm[2 * (threadIdx.x >> 6) + 1] = s2;
-        }
-        __syncthreads();
-        s1 = s2 = 0.0f;
-        for (int i = 0; i < (int)(blockDim.x >> 6); ++i) {
-          s1 += sm[2 * i];
-          s2 += sm[2 * i + 1];
-        }
-      } else {
-        s1 = K > 1 ? wave64_sum(s1) : lanes_sum(s1, shift);
-        s2 = K > 1 ? wave64_sum(s2) : lanes_sum(s2, shift);
-      }
-      const float c1 = s1 * inv, c2 = s2 * inv;
-      if (row < a.rows) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          if (nv[k] <= 0) continue;
-          const long long at = row * a.cols + (k * lanes + tl) * 8;
-          float dz[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) dz[j] = rstd[u] * (fmaf(vd[u][k].get(j), w[k][j], -c1) - xh[k][j] * c2);
-          if (RES && a.dresidual != nullptr) {
-            Vec8<TR> o;
-            o.set(dz);
-            o.store(reinterpret_cast<TR*>(a.dresidual) + at, nv[k]);
-          }
-          if (a.dx != nullptr) {
-            if (RES && a.drop.on) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) dz[j] = (m[k] >> j & 1) ? dz[j] * a.drop.scale : 0.0f;
-            }
-            Vec8<TX> o;
-            o.set(dz);
-            o.store(reinterpret_cast<TX*>(a.dx) + at, nv[k]);
-          }
-        }
-      }
-    }
+  };
+  const long long step = (long long)gridDim.x * teams;
+  long long base = (long long)blockIdx.x * teams;
+  if (base < a.rows) load(base);
+  for (; base < a.rows; base += step) {
+    const long long row = base + team;
+    float xh[K][8], g[K][8], s1, s2;
+    Keep8 m[K];
+    const float rstd = in.rstd;
+    bwd_row<TX, TR, RES, K>(a, key, in, sp, row >= a.rows, row, lanes, tl, K > 1 ? red : w, xh, g, m, dw, db, s1, s2);
+    if (base + step < a.rows) load(base + step);
+    const float c1 = lanes_sum(s1, shift) * inv, c2 = lanes_sum(s2, shift) * inv;
+    if (row < a.rows) bwd_put<TX, TR, RES, K>(a, sp, row * a.cols, lanes, tl, c1, c2, rstd, xh, g, m);
   }
   if (a.dweight == nullptr && a.dbias == nullptr) return;
-  if (BLK) {
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < nv[k]) {
-          put_part<TX>(a, 0, (k * lanes + tl) * 8 + j, dw[k][j]);
-          put_part<TX>(a, 1, (k * lanes + tl) * 8 + j, db[k][j]);
-        }
-    return;
-  }
   // the teams of a wave, then the four waves
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     float(&acc)[K][8] = which == 0 ? dw : db;
-    if (K == 1) {
-      for (int s = lanes; s < 64; s <<= 1)
+    for (int s = lanes; s < 64; s <<= 1)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[0][j] += __shfl_xor(acc[0][j], s);
-    }
-    if (which == 1) __syncthreads();
-    const int wave = threadIdx.x >> 6;
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[k][j] += __shfl_xor(acc[k][j], s);
+    if (K > 1 || which == 1) __syncthreads();
     if ((int)(threadIdx.x & 63) < lanes) {
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) red[wave * (512 * K) + (k * lanes + tl) * 8 + j] = acc[k][j];
+        for (int j = 0; j < 8; ++j) red[(threadIdx.x >> 6) * (512 * K) + (k * lanes + tl) * 8 + j] = acc[k][j];
     }
     __syncthreads();
     for (int c = threadIdx.x; c < cols; c += 256)
       put_part<TX>(a, which, c, (red[c] + red[512 * K + c]) + (red[2 * 512 * K + c] + red[3 * 512 * K + c]));
   }
+}
+
+// Rows of a workgroup.  AHEAD: the next row's loads pass behind this row's sums, as above, at the price of registers (512 threads at
+// most); otherwise up to 1024 threads with 128 registers each, a row at a time.
+template <class TX, class TR, int RES, int K, bool AHEAD>
+__global__ __launch_bounds__(AHEAD ? 512 : 1024) void norm_bwd_block_kernel(NormArgs a) {
+  extern __shared__ __align__(16) float wlds[];            // K * blockDim.x * 8 weights
+  __shared__ float sums[2][16][2];
+  const int lanes = blockDim.x, tl = threadIdx.x, cols = (int)a.cols;
+  const float inv = 1.0f / (float)cols;
+  DropKey key{};
+  if (RES) key = drop_key(a.drop);
+  Span sp[K];
+  float dw[K][8] = {}, db[K][8] = {};
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    float w[8];
+    sp[k] = Span((k * lanes + tl) * 8, cols);
+    load_param<TX>(a.weight, a.p_f32, sp[k], 1.0f, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) wlds[(k * lanes + tl) * 8 + j] = w[j];      // read by this thread only
+  }
+  BwdRow<TX, TR, K> in;
+  const auto load = [&](long long row) {
+    const TX* px = reinterpret_cast<const TX*>(a.x) + row * a.ld_x;
+    const TR* pr = reinterpret_cast<const TR*>(a.residual) + row * a.ld_r;
+    const TR* pd = reinterpret_cast<const TR*>(a.dy) + row * a.ld_dy;
+    in.mean = a.mean[row];
+    in.rstd = a.rstd[row];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      in.d[k].load(pd + sp[k].at);
+      in.x[k].load(px + sp[k].at);
+      if (RES) in.r[k].load(pr + sp[k].at);
+    }
+  };
+  if (AHEAD && blockIdx.x < a.rows) load(blockIdx.x);
+  int half = 0;
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    if (!AHEAD) load(row);
+    float xh[K][8], g[K][8], s1, s2;
+    Keep8 m[K];
+    const float rstd = in.rstd;
+    bwd_row<TX, TR, RES, K>(a, key, in, sp, false, row, lanes, tl, wlds, xh, g, m, dw, db, s1, s2);
+    if (AHEAD && row + gridDim.x < a.rows) load(row + gridDim.x);
+    // one barrier a row: the next row writes the other half, and the one after it finds every thread past this row's reads
+    s1 = wave64_sum(s1);
+    s2 = wave64_sum(s2);
+    if ((tl & 63) == 0) {
+      sums[half][tl >> 6][0] = s1;
+      sums[half][tl >> 6][1] = s2;
+    }
+    __syncthreads();
+    s1 = s2 = 0.0f;
+    for (int i = 0; i < lanes >> 6; ++i) {
+      s1 += sums[half][i][0];
+      s2 += sums[half][i][1];
+    }
+    half ^= 1;
+    bwd_put<TX, TR, RES, K>(a, sp, row * a.cols, lanes, tl, s1 * inv, s2 * inv, rstd, xh, g, m);
+  }
+  if (a.dweight == nullptr && a.dbias == nullptr) return;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < 8 - sp[k].cut) {
+        put_part<TX>(a, 0, (k * lanes + tl) * 8 + j, dw[k][j]);
+        put_part<TX>(a, 1, (k * lanes + tl) * 8 + j, db[k][j]);
+      }
 }
 
 // dweight / dbias = the partial sums added up in a fixed order: 32 columns x 32 slices of the partial sums a workgroup
@@ -207,27 +272,39 @@ int norm_finish(const NormArgs& a, int parts, hipStream_t s) {
   return check_launch("norm_backward");
 }
 
-static int rows_at_once(const NormShape& sh) { return sh.block ? 1 : sh.k == 1 ? NB_U1 : sh.k == 2 ? NB_U2 : 1; }
-// workgroups = partial sums
-static int norm_parts(long long rows, const NormShape& sh) {
-  const long long per = (long long)sh.teams() * rows_at_once(sh);
-  long long g = (rows + per - 1) / per;
-  const long long most = sh.block ? NB_GB * 512 / sh.threads : NB_G;
+// The teams of the backward pass: more than 1024 columns belong to a workgroup (K = 4 in a wave leaves one wave a SIMD), more than 4096 to
+// K = 4 chunks a thread where those and the loads ahead fit 256 registers: half precision without a residual.
+static NormShape bwd_shape(long long cols, bool lean) {
+  const int chunks = (int)((cols + 7) / 8);
+  if (chunks <= 128) return norm_shape(cols);
+  NormShape s{chunks > 512 && lean ? 4 : 2, 0, 0, true};
+  s.threads = (chunks + 64 * s.k - 1) / (64 * s.k) * 64;
+  return s;
+}
+// workgroups = partial sums; no type changes their number
+static int norm_parts(long long rows, long long cols) {
+  const NormShape sh = bwd_shape(cols, false);
+  const long long g = (rows + sh.teams() - 1) / sh.teams();
+  const long long most = !sh.block ? NB_G : 256 * (sh.threads <= 128 ? 3 : sh.threads <= 256 ? 2 : 1);
   return (int)(g < 1 ? 1 : g < most ? g : most);
 }
 
 uint64_t norm_workspace_bytes(long long rows, long long cols) {
-  const int parts = cols > kNormRowMax ? norm_wide_parts(rows, cols) : norm_parts(rows, norm_shape(cols));
+  const int parts = cols < kNormRowMin || cols > kNormRowMax ? norm_wide_parts(rows, cols) : norm_parts(rows, cols);
   return (uint64_t)parts * 2 * (uint64_t)cols * sizeof(float);
 }
 
 template <class TX, class TR, int RES> static int backward(const NormArgs& a, hipStream_t s) {
-  const NormShape sh = norm_shape(a.cols);
-  const int grid = norm_parts(a.rows, sh);
-  if (sh.block) norm_bwd_kernel<TX, TR, RES, 2, 1, true><<<grid, sh.threads, 0, s>>>(a, 0);
-  else if (sh.k == 1) norm_bwd_kernel<TX, TR, RES, 1, NB_U1, false><<<grid, 256, 0, s>>>(a, sh.shift);
-  else if (sh.k == 2) norm_bwd_kernel<TX, TR, RES, 2, NB_U2, false><<<grid, 256, 0, s>>>(a, 6);
-  else norm_bwd_kernel<TX, TR, RES, 4, 1, false><<<grid, 256, 0, s>>>(a, 6);
+  const NormShape sh = bwd_shape(a.cols, RES == 0 && sizeof(TX) == 2);
+  const int grid = norm_parts(a.rows, a.cols);
+  const size_t lds = (size_t)sh.threads * sh.k * 8 * sizeof(float);
+  if (sh.block && sh.k == 4) norm_bwd_block_kernel<TX, TR, RES, RES == 0 && sizeof(TX) == 2 ? 4 : 2, true><<<grid, sh.threads, lds, s>>>(a);
+  else if (sh.block && sh.threads <= 256) norm_bwd_block_kernel<TX, TR, RES, 2, true><<<grid, sh.threads, lds, s>>>(a);
+  else if (sh.block) norm_bwd_block_kernel<TX, TR, RES, 2, false><<<grid, sh.threads, lds, s>>>(a);
+  else if (sh.k == 1) norm_bwd_kernel<TX, TR, RES, 1><<<grid, 256, 0, s>>>(a, sh.shift);
+  else if (sh.k == 2) norm_bwd_kernel<TX, TR, RES, 2><<<grid, 256, 0, s>>>(a, sh.shift);
+  else if (sh.k == 3) norm_bwd_kernel<TX, TR, RES, 3><<<grid, 256, 0, s>>>(a, sh.shift);
+  else norm_bwd_kernel<TX, TR, RES, 4><<<grid, 256, 0, s>>>(a, sh.shift);
   if (check_launch("norm_backward")) return -1;
   if (grid > 1 && (a.dweight != nullptr || a.dbias != nullptr)) return norm_finish(a, grid, s);
   return 0;
@@ -236,7 +313,7 @@ template <class TX, class TR, int RES> static int backward(const NormArgs& a, hi
 int norm_backward(const NormArgs& a, hipStream_t stream) {
   ProfScope prof("norm_backward", stream, 14.0 * a.rows * a.cols,
                  (double)a.rows * a.cols * (2.0 * elem_size(a.x_type) + elem_size(a.y_type) * (a.residual ? 3.0 : 1.0)));
-  if (a.cols > kNormRowMax) return norm_wide_backward(a, stream);
+  if (a.cols < kNormRowMin || a.cols > kNormRowMax) return norm_wide_backward(a, stream);
   NORM_DISPATCH(backward, a, stream);
 }
 

@@ -1,118 +1,187 @@
 // Layer normalisation with the row in registers: y = (z - mean) rstd w + b, z = x or residual + dropout(x).
 // One sweep over memory: a team of threads (norm.hpp) loads its row, sums it, sums the squared deviations from that mean (the two-pass
-// form: no cancellation however large the mean) and writes y.  Bound by HBM: x (and residual) in, y out.  U rows a team are loaded before
-// the first is used, and a workgroup ends after them: a grid in row order keeps the whole chip on neighbouring pages.
+// form: no cancellation however large the mean) and writes y.  Bound by HBM: x (and residual) in, y out.
 #include "norm.hpp"
 
 namespace lbm {
 
-template <class TX, class TR, int RES, int K, int U, bool BLK>
-__global__ __launch_bounds__(BLK ? 1024 : 256) void norm_fwd_kernel(NormArgs a, int shift) {
-  __shared__ float sm[2][16];
-  const int lanes = BLK ? blockDim.x : K > 1 ? 64 : 1 << shift;
-  const int tl = BLK ? threadIdx.x : threadIdx.x & (lanes - 1);
-  const int team = BLK ? 0 : K > 1 ? threadIdx.x >> 6 : threadIdx.x >> shift;
-  const int teams = BLK ? 1 : K > 1 ? 4 : 256 >> shift;
-  const int cols = (int)a.cols;
+template <class TX, class TR, int K> struct FwdRow {
+  Vec8<TX> x[K];
+  Vec8<TR> r[K];
+};
+
+// z of a loaded row, its sum in s
+template <class TX, class TR, int RES, int K>
+__device__ __forceinline__ float join_row(const NormArgs& a, const DropKey& key, FwdRow<TX, TR, K>& in, const Span (&sp)[K], long long row,
+                                          int lanes, int tl, float (&z)[K][8]) {
+  float s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    in.x[k].cut(sp[k].cut);
+    if (RES) in.r[k].cut(sp[k].cut);
+    if (RES && a.drop.on) {
+      const Keep8 m = keep8((uint64_t)(row * a.cols + (k * lanes + tl) * 8), key, a.drop.tm1);
+      const uint32_t limit = keep_limit(a.drop.tm1);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[k][j] = join_one<RES>(in.x[k].get(j), in.r[k].get(j), m.kept(j, limit), a.drop.scale);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[k][j] = join_one<RES>(in.x[k].get(j), RES ? in.r[k].get(j) : 0.0f, true, 1.0f);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += z[k][j];              // what was cut is zero
+  }
+  return s;
+}
+// z -= mean; the sum of its squares over the elements that exist
+template <int K> __device__ __forceinline__ float deviate(float (&z)[K][8], float mean, const Span (&sp)[K]) {
+  float s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) z[k][j] -= mean;
+    if (sp[k].cut != 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[k][j] = j < 8 - sp[k].cut ? z[k][j] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fmaf(z[k][j], z[k][j], s);
+  }
+  return s;
+}
+template <class TR> __device__ __forceinline__ void put_y(TR* y, float (&z)[8], float rstd, const float (&w)[8], const float (&b)[8], int cut) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) z[j] = fmaf(z[j] * rstd, w[j], b[j]);
+  Vec8<TR> o;
+  o.set(z);
+  o.store(y, 8 - cut);
+}
+
+// Rows of up to 2048 columns.  U rows a team are loaded before the first is used, and a workgroup ends after them: a grid in row order
+// keeps the whole chip on neighbouring pages.
+template <class TX, class TR, int RES, int K, int U>
+__global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift) {
+  const int lanes = 1 << shift, tl = threadIdx.x & (lanes - 1), team = threadIdx.x >> shift, teams = 256 >> shift, cols = (int)a.cols;
   const float inv = 1.0f / (float)cols;
   DropKey key{};
   if (RES) key = drop_key(a.drop);
-  int nv[K];
+  Span sp[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) nv[k] = min(8, cols - (k * lanes + tl) * 8);
-  for (long long base = (long long)blockIdx.x * (teams * U); base < a.rows; base += (long long)gridDim.x * (teams * U)) {
-    Vec8<TX> vx[U][K];
-    Vec8<TR> vr[U][K];
+  for (int k = 0; k < K; ++k) sp[k] = Span((k * lanes + tl) * 8, cols);
+  const long long base = (long long)blockIdx.x * (teams * U);
+  const int last = (int)min((long long)(teams * U), a.rows - base) - 1;          // of this workgroup's rows
+  const TX* px = reinterpret_cast<const TX*>(a.x) + base * a.ld_x;
+  const TR* pr = reinterpret_cast<const TR*>(a.residual) + base * a.ld_r;
+  TR* py = reinterpret_cast<TR*>(a.y) + base * a.cols;
+  FwdRow<TX, TR, K> in[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long long row = base + u * teams + team;
-      const bool in = row < a.rows;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int c = (k * lanes + tl) * 8, n = in ? nv[k] : 0;
-        vx[u][k].load(reinterpret_cast<const TX*>(a.x) + row * a.ld_x + c, n);
-        if (RES) vr[u][k].load(reinterpret_cast<const TR*>(a.residual) + row * a.ld_r + c, n);
-      }
-    }
-    float w[K][8], b[K][8];
+  for (int u = 0; u < U; ++u) {
+    const uint32_t r = min(u * teams + team, last);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      load_param<TX>(a.weight, a.p_f32, (k * lanes + tl) * 8, nv[k], 1.0f, w[k]);
-      load_param<TX>(a.bias, a.p_f32, (k * lanes + tl) * 8, nv[k], 0.0f, b[k]);
+      in[u].x[k].load(px + row_at(r, (uint32_t)a.ld_x, sp[k].at));
+      if (RES) in[u].r[k].load(pr + row_at(r, (uint32_t)a.ld_r, sp[k].at));
+    }
+  }
+  float w[K][8], b[K][8];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    load_param<TX>(a.weight, a.p_f32, sp[k], 1.0f, w[k]);
+    load_param<TX>(a.bias, a.p_f32, sp[k], 0.0f, b[k]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int r = u * teams + team;
+    float z[K][8];
+    const float mean = lanes_sum(join_row<TX, TR, RES, K>(a, key, in[u], sp, base + r, lanes, tl, z), shift) * inv;
+    const float rstd = rsqrt_newton(lanes_sum(deviate<K>(z, mean, sp), shift) * inv + a.eps);
+    if (r > last) continue;
+    if (tl == 0 && a.mean != nullptr) {
+      a.mean[base + r] = mean;
+      a.rstd[base + r] = rstd;
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long long row = base + u * teams + team;
-      float z[K][8], s = 0.0f;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        uint32_t m = 0xffu;
-        float scale = 1.0f;
-        if (RES && a.drop.on) {
-          m = keep8((uint64_t)(row * a.cols + (k * lanes + tl) * 8), key, a.drop.tm1);
-          scale = a.drop.scale;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          z[k][j] = join_one<RES>(vx[u][k].get(j), RES ? vr[u][k].get(j) : 0.0f, m >> j & 1, scale);
-          s += z[k][j];                                    // elements past the row's end were loaded as zeros
-        }
-      }
-      const float mean = (BLK ? block_sum(s, sm[0]) : K > 1 ? wave64_sum(s) : lanes_sum(s, shift)) * inv;
-      s = 0.0f;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) z[k][j] -= mean;
-        if (nv[k] < 8) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) z[k][j] = j < nv[k] ? z[k][j] : 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s = fmaf(z[k][j], z[k][j], s);
-      }
-      const float var = (BLK ? block_sum(s, sm[1]) : K > 1 ? wave64_sum(s) : lanes_sum(s, shift)) * inv;
-      const float rstd = 1.0f / sqrtf(var + a.eps);
-      if (row < a.rows) {
-        if (tl == 0 && a.mean != nullptr) {
-          a.mean[row] = mean;
-          a.rstd[row] = rstd;
-        }
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          if (nv[k] <= 0) continue;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) z[k][j] = fmaf(z[k][j] * rstd, w[k][j], b[k][j]);
-          Vec8<TR> o;
-          o.set(z[k]);
-          o.store(reinterpret_cast<TR*>(a.y) + row * a.cols + (k * lanes + tl) * 8, nv[k]);
-        }
-      }
-    }
+    for (int k = 0; k < K; ++k)
+      if (sp[k].cut < 8) put_y<TR>(py + row_at(r, (uint32_t)cols, (k * lanes + tl) * 8), z[k], rstd, w[k], b[k], sp[k].cut);
   }
 }
 
-#ifndef NF_U1
-#define NF_U1 2
-#define NF_U2 1
+// Rows of a workgroup.  The next row's loads are issued when this row has become z, so they pass behind its two sums and its stores: with
+// 512 or 1024 threads a row only one or two rows are on a CU, and without that its memory was idle half of the time.
+template <class TX, class TR, int RES, int K>
+__global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
+  __shared__ float sm[2][16];
+  const int lanes = blockDim.x, tl = threadIdx.x, cols = (int)a.cols;
+  const float inv = 1.0f / (float)cols;
+  DropKey key{};
+  if (RES) key = drop_key(a.drop);
+  Span sp[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) sp[k] = Span((k * lanes + tl) * 8, cols);
+  FwdRow<TX, TR, K> in;
+  const auto load = [&](long long row) {
+    const TX* px = reinterpret_cast<const TX*>(a.x) + row * a.ld_x;
+    const TR* pr = reinterpret_cast<const TR*>(a.residual) + row * a.ld_r;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      in.x[k].load(px + sp[k].at);
+      if (RES) in.r[k].load(pr + sp[k].at);
+    }
+  };
+  float w[K][8], b[K][8];
+  load(blockIdx.x);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    load_param<TX>(a.weight, a.p_f32, sp[k], 1.0f, w[k]);
+    load_param<TX>(a.bias, a.p_f32, sp[k], 0.0f, b[k]);
+  }
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    float z[K][8];
+    const float s = join_row<TX, TR, RES, K>(a, key, in, sp, row, lanes, tl, z);
+    if (row + gridDim.x < a.rows) load(row + gridDim.x);
+    const float mean = block_sum(s, sm[0]) * inv;
+    const float rstd = rsqrt_newton(block_sum(deviate<K>(z, mean, sp), sm[1]) * inv + a.eps);
+    if (tl == 0 && a.mean != nullptr) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+    TR* py = reinterpret_cast<TR*>(a.y) + row * a.cols;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (sp[k].cut < 8) put_y<TR>(py + (k * lanes + tl) * 8, z[k], rstd, w[k], b[k], sp[k].cut);
+  }
+}
+
+#ifndef NF_GB
+#define NF_GB 512
+#define NF_MANY 2048
 #endif
+template <class TX, class TR, int RES, int K, int U> static int wave_forward(const NormArgs& a, const NormShape& sh, hipStream_t s) {
+  const long long per = (long long)sh.teams() * U, grid = (a.rows + per - 1) / per;
+  LBM_REQUIRE(grid < (1ll << 31), "norm_forward: %lld rows are more than a grid holds", a.rows);
+  norm_fwd_kernel<TX, TR, RES, K, U><<<(unsigned)grid, 256, 0, s>>>(a, sh.shift);
+  return check_launch("norm_forward");
+}
 template <class TX, class TR, int RES> static int forward(const NormArgs& a, hipStream_t s) {
   const NormShape sh = norm_shape(a.cols);
-  const int u = sh.block ? 1 : sh.k == 1 ? NF_U1 : sh.k == 2 ? NF_U2 : 1;
-  const long long per = (long long)sh.teams() * u, want = (a.rows + per - 1) / per;
-  const unsigned grid = (unsigned)(want < (1ll << 30) ? want : (1ll << 30));
-  if (sh.block) norm_fwd_kernel<TX, TR, RES, 2, 1, true><<<grid, sh.threads, 0, s>>>(a, 0);
-  else if (sh.k == 1) norm_fwd_kernel<TX, TR, RES, 1, NF_U1, false><<<grid, 256, 0, s>>>(a, sh.shift);
-  else if (sh.k == 2) norm_fwd_kernel<TX, TR, RES, 2, NF_U2, false><<<grid, 256, 0, s>>>(a, 6);
-  else norm_fwd_kernel<TX, TR, RES, 4, 1, false><<<grid, 256, 0, s>>>(a, 6);
-  return check_launch("norm_forward");
+  if (sh.block) {
+    const long long most = NF_GB * 512 / sh.threads;
+    norm_fwd_block_kernel<TX, TR, RES, 2><<<(unsigned)(a.rows < most ? a.rows : most), sh.threads, 0, s>>>(a);
+    return check_launch("norm_forward");
+  }
+  constexpr int U1 = RES ? 2 : 4, U2 = RES ? 1 : 2;
+  if (sh.k == 4) return wave_forward<TX, TR, RES, 4, 1>(a, sh, s);
+  const bool many = a.rows >= (long long)sh.teams() * (sh.k == 1 ? U1 : U2) * NF_MANY;
+  if (sh.k == 1) return many ? wave_forward<TX, TR, RES, 1, U1>(a, sh, s) : wave_forward<TX, TR, RES, 1, 1>(a, sh, s);
+  if (sh.k == 2) return many ? wave_forward<TX, TR, RES, 2, U2>(a, sh, s) : wave_forward<TX, TR, RES, 2, 1>(a, sh, s);
+  return many ? wave_forward<TX, TR, RES, 3, U2>(a, sh, s) : wave_forward<TX, TR, RES, 3, 1>(a, sh, s);
 }
 
 int norm_forward(const NormArgs& a, hipStream_t stream) {
   if (a.rows == 0) return 0;
   ProfScope prof("norm_forward", stream, 8.0 * a.rows * a.cols,
                  (double)a.rows * a.cols * (elem_size(a.x_type) + elem_size(a.y_type) * (a.residual ? 2.0 : 1.0)));
-  if (a.cols > kNormRowMax) return norm_wide_forward(a, stream);
+  if (a.cols < kNormRowMin || a.cols > kNormRowMax) return norm_wide_forward(a, stream);
   NORM_DISPATCH(forward, a, stream);
 }
 

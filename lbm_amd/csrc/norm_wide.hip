@@ -9,6 +9,36 @@
 
 namespace lbm {
 
+template <class T> __device__ __forceinline__ void load_nv(Vec8<T>& v, const T* p, int nv) {
+  if (nv == 8) v.load(p);
+  else v.load_some(p, nv);
+}
+// weight / bias as fp32 (absent: `dflt`)
+template <class TX> __device__ __forceinline__ void load_param_some(const void* p, int p_f32, long long c, int nv, float dflt, float (&v)[8]) {
+  Vec8<float> f;
+  Vec8<TX> h;
+  if (p != nullptr) {
+    if (p_f32) load_nv(f, reinterpret_cast<const float*>(p) + c, nv);
+    else load_nv(h, reinterpret_cast<const TX*>(p) + c, nv);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = p == nullptr ? dflt : p_f32 ? f.get(j) : h.get(j);
+}
+// the eight z values of a chunk; true where something may be dropped (then m says which)
+template <class TX, class TR, int RES>
+__device__ __forceinline__ bool load_z(const NormArgs& a, const DropKey& key, long long row, long long c, int nv, float (&z)[8], Keep8& m) {
+  Vec8<TX> vx;
+  Vec8<TR> vr;
+  load_nv(vx, reinterpret_cast<const TX*>(a.x) + row * a.ld_x + c, nv);
+  if (RES) load_nv(vr, reinterpret_cast<const TR*>(a.residual) + row * a.ld_r + c, nv);
+  const bool drop = RES && a.drop.on;
+  if (drop) m = keep8((uint64_t)(row * a.cols + c), key, a.drop.tm1);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    z[j] = join_one<RES>(vx.get(j), RES ? vr.get(j) : 0.0f, !drop || m.kept(j, keep_limit(a.drop.tm1)), drop ? a.drop.scale : 1.0f);
+  return drop;
+}
+
 template <class TX, class TR, int RES>
 __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
   __shared__ float sm[2][16];
@@ -16,9 +46,10 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
   if (RES) key = drop_key(a.drop);
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     float s = 0.0f, z[8];
+    Keep8 m;
     for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
       const int nv = (int)min(8ll, a.cols - c);
-      load_z<TX, TR, RES>(a, key, row, c, nv, z);
+      load_z<TX, TR, RES>(a, key, row, c, nv, z, m);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s += j < nv ? z[j] : 0.0f;
     }
@@ -26,7 +57,7 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
     s = 0.0f;
     for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
       const int nv = (int)min(8ll, a.cols - c);
-      load_z<TX, TR, RES>(a, key, row, c, nv, z);
+      load_z<TX, TR, RES>(a, key, row, c, nv, z, m);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s += j < nv ? (z[j] - mean) * (z[j] - mean) : 0.0f;
     }
@@ -38,9 +69,9 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
     for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
       const int nv = (int)min(8ll, a.cols - c);
       float w[8], b[8];
-      load_z<TX, TR, RES>(a, key, row, c, nv, z);
-      load_param<TX>(a.weight, a.p_f32, c, nv, 1.0f, w);
-      load_param<TX>(a.bias, a.p_f32, c, nv, 0.0f, b);
+      load_z<TX, TR, RES>(a, key, row, c, nv, z, m);
+      load_param_some<TX>(a.weight, a.p_f32, c, nv, 1.0f, w);
+      load_param_some<TX>(a.bias, a.p_f32, c, nv, 0.0f, b);
 #pragma unroll
       for (int j = 0; j < 8; ++j) z[j] = fmaf((z[j] - mean) * rstd, w[j], b[j]);
       Vec8<TR> o;
@@ -58,12 +89,13 @@ __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const float mean = a.mean[row], rstd = a.rstd[row];
     float s1 = 0.0f, s2 = 0.0f, z[8], w[8];
+    Keep8 m;
     for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
       const int nv = (int)min(8ll, a.cols - c);
-      load_z<TX, TR, RES>(a, key, row, c, nv, z);
-      load_param<TX>(a.weight, a.p_f32, c, nv, 1.0f, w);
+      load_z<TX, TR, RES>(a, key, row, c, nv, z, m);
+      load_param_some<TX>(a.weight, a.p_f32, c, nv, 1.0f, w);
       Vec8<TR> d;
-      d.load(reinterpret_cast<const TR*>(a.dy) + row * a.ld_dy + c, nv);
+      load_nv(d, reinterpret_cast<const TR*>(a.dy) + row * a.ld_dy + c, nv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float g = d.get(j) * w[j];
@@ -74,10 +106,10 @@ __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
     const float c1 = block_sum(s1, sm[0]) / (float)a.cols, c2 = block_sum(s2, sm[1]) / (float)a.cols;
     for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
       const int nv = (int)min(8ll, a.cols - c);
-      const uint32_t m = load_z<TX, TR, RES>(a, key, row, c, nv, z);
-      load_param<TX>(a.weight, a.p_f32, c, nv, 1.0f, w);
+      const bool drop = load_z<TX, TR, RES>(a, key, row, c, nv, z, m);
+      load_param_some<TX>(a.weight, a.p_f32, c, nv, 1.0f, w);
       Vec8<TR> d;
-      d.load(reinterpret_cast<const TR*>(a.dy) + row * a.ld_dy + c, nv);
+      load_nv(d, reinterpret_cast<const TR*>(a.dy) + row * a.ld_dy + c, nv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) z[j] = rstd * (d.get(j) * w[j] - c1 - (z[j] - mean) * rstd * c2);
       if (RES && a.dresidual != nullptr) {
@@ -85,9 +117,9 @@ __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
         d.store(reinterpret_cast<TR*>(a.dresidual) + row * a.cols + c, nv);
       }
       if (a.dx != nullptr) {
-        if (RES && a.drop.on) {
+        if (drop) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) z[j] = (m >> j & 1) ? z[j] * a.drop.scale : 0.0f;
+          for (int j = 0; j < 8; ++j) z[j] = m.kept(j, keep_limit(a.drop.tm1)) ? z[j] * a.drop.scale : 0.0f;
         }
         Vec8<TX> o;
         o.set(z);
@@ -106,11 +138,12 @@ __global__ __launch_bounds__(256) void norm_wide_dw_kernel(NormArgs a) {
   if (c >= a.cols) return;
   const int nv = (int)min(8ll, a.cols - c);
   float dw[8] = {}, db[8] = {}, z[8];
+  Keep8 m;
   for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
     const float mean = a.mean[row], rstd = a.rstd[row];
-    load_z<TX, TR, RES>(a, key, row, c, nv, z);
+    load_z<TX, TR, RES>(a, key, row, c, nv, z, m);
     Vec8<TR> d;
-    d.load(reinterpret_cast<const TR*>(a.dy) + row * a.ld_dy + c, nv);
+    load_nv(d, reinterpret_cast<const TR*>(a.dy) + row * a.ld_dy + c, nv);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       dw[j] = fmaf(d.get(j), (z[j] - mean) * rstd, dw[j]);

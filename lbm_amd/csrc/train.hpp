@@ -30,14 +30,16 @@ __device__ __forceinline__ DropKey drop_key(const DropArgs& d) {
 }
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-// Philox4x32 with ten rounds (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", SC 2011)
+// Philox4x32 with ten rounds (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", SC 2011).  A round is two
+// v_mad_u64_u32 and two three-input exclusive ors; ten of them are what dropout computes, and stay below what it reads and writes.
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
 __device__ __forceinline__ u32x4 philox(uint64_t n, DropKey k) {
   uint32_t c0 = (uint32_t)n, c1 = (uint32_t)(n >> 32), c2 = k.o0, c3 = k.o1;
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k.k0;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k.k1;
+    c0 = xor3((uint32_t)(b >> 32), c1, k.k0);
+    c2 = xor3((uint32_t)(a >> 32), c3, k.k1);
     c1 = (uint32_t)b;
     c3 = (uint32_t)a;
     k.k0 += 0x9E3779B9u;
@@ -45,73 +47,124 @@ __device__ __forceinline__ u32x4 philox(uint64_t n, DropKey k) {
   }
   return u32x4{c0, c1, c2, c3};
 }
-// bit j: element 8 block + j is kept
-__device__ __forceinline__ uint32_t block_keep(uint64_t block, const DropKey& k, uint32_t tm1) {
-  const uint32_t th = tm1 >> 16, tl = tm1 & 0xffffu;
-  const u32x4 w = philox(2 * block, k);
-  uint32_t keep = 0;
-  bool tie = false;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t h = (j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu;
-    keep |= h > th ? 1u << j : 0u;
-    tie |= h == th;
+
+// Eight elements' decisions: eight 16-bit numbers, an element is kept where its number is above `limit`.  Elements whose upper half
+// ties with the threshold's are decided by the lower halves and then set to 0xffff or 0; limit is at most 0xfffe, so 0xffff is above it.
+struct Keep8 {
+  u32x4 w;
+  __device__ __forceinline__ bool kept(int j, uint32_t limit) const {
+    const uint32_t v = w[j >> 1];
+    return (j & 1) ? v > (limit << 16 | 0xffffu) : (uint16_t)v > (uint16_t)limit;
   }
-  if (tie) {
-    const u32x4 l = philox(2 * block + 1, k);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t h = (j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu;
-      const uint32_t q = (j & 1) ? l[j >> 1] >> 16 : l[j >> 1] & 0xffffu;
-      keep |= h == th && q > tl ? 1u << j : 0u;
-    }
-  }
-  return keep;
+};
+__device__ __forceinline__ uint32_t keep_limit(uint32_t tm1) { return min(tm1 >> 16, 0xfffeu); }
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pk_min(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
-// the same for eight elements that start anywhere: a row whose length is no multiple of eight straddles two blocks
-__device__ __forceinline__ uint32_t keep8(uint64_t e, const DropKey& k, uint32_t tm1) {
+// does any of the eight halves equal the threshold's upper half?
+__device__ __forceinline__ bool any_tie(const u32x4& w, uint32_t tm1) {
+  const uint32_t hh = (tm1 >> 16) * 0x10001u;
+  const uint32_t w0 = w[0] ^ hh, w1 = w[1] ^ hh, w2 = w[2] ^ hh, w3 = w[3] ^ hh;
+  const uint32_t m = pk_min(pk_min(w0, w1), pk_min(w2, w3));
+  return (m & 0xffffu) == 0 || m < 0x10000u;
+}
+__device__ __forceinline__ void settle_ties(u32x4& w, const u32x4& low, uint32_t tm1) {
+  const uint32_t th = tm1 >> 16, tl = tm1 & 0xffffu;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t lo = w[i] & 0xffffu, hi = w[i] >> 16;
+    if (lo == th) lo = (low[i] & 0xffffu) > tl ? 0xffffu : 0u;
+    if (hi == th) hi = (low[i] >> 16) > tl ? 0xffffu : 0u;
+    w[i] = hi << 16 | lo;
+  }
+}
+__device__ __forceinline__ Keep8 block_keep(uint64_t block, const DropKey& k, uint32_t tm1) {
+  Keep8 m{philox(2 * block, k)};
+  if (any_tie(m.w, tm1)) settle_ties(m.w, philox(2 * block + 1, k), tm1);
+  return m;
+}
+// eight 16-bit numbers from slot sh (1 .. 7) of block a on into block b
+__device__ __forceinline__ u32x4 straddle(const u32x4& a, const u32x4& b, uint32_t sh) {
+  u32x4 p = a, q = b;
+  if (sh & 4) {
+    p = u32x4{a[2], a[3], b[0], b[1]};
+    q = u32x4{b[2], b[3], 0, 0};
+  }
+  if (sh & 2) {
+    p = u32x4{p[1], p[2], p[3], q[0]};
+    q[0] = q[1];
+  }
+  if (sh & 1) p = u32x4{p[0] >> 16 | p[1] << 16, p[1] >> 16 | p[2] << 16, p[2] >> 16 | p[3] << 16, p[3] >> 16 | q[0] << 16};
+  return p;
+}
+// the eight elements from e on; rows whose length is no multiple of eight start anywhere in a block
+__device__ __forceinline__ Keep8 keep8(uint64_t e, const DropKey& k, uint32_t tm1) {
   const uint32_t sh = (uint32_t)e & 7u;
-  uint32_t m = block_keep(e >> 3, k, tm1);
-  if (sh != 0) m = (m | block_keep((e >> 3) + 1, k, tm1) << 8) >> sh;
+  const uint64_t b = e >> 3;
+  Keep8 m{philox(2 * b, k)};
+  if (sh != 0) m.w = straddle(m.w, philox(2 * b + 2, k), sh);
+  if (any_tie(m.w, tm1)) {
+    u32x4 low = philox(2 * b + 1, k);
+    if (sh != 0) low = straddle(low, philox(2 * b + 3, k), sh);
+    settle_ties(m.w, low, tm1);
+  }
   return m;
 }
 
 // ---- eight consecutive elements of a row ---------------------------------------------------------------------------
 // One 16-byte access (two for fp32) at any element alignment: gfx950 serves unaligned global accesses, an odd row length costs only the
-// second cache line that some of them touch.  nv = how many of the eight exist (>= 8: all).
+// second cache line that some of them touch (1024 columns at a stride of 1025: 5 % off the aligned time).
+//   load           eight elements; near a row's end the caller reads earlier ones and cuts (below)
+//   load_some      the first nv of eight, element by element
+//   cut(s)         drops the first s elements and fills up with zeros (s = 8: all zeros)
+//   store(p, nv)   the first nv of eight
 template <class T> struct Vec8;
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
 typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
+typedef u32x2 u32x2_a4 __attribute__((aligned(4)));
+typedef uint32_t u32_a2 __attribute__((aligned(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 template <> struct Vec8<float> {
   u32x4 a, b;
-  __device__ __forceinline__ void load(const float* p, int nv) {
-    if (nv >= 8) {
-      a = *reinterpret_cast<const u32x4_a4*>(p);
-      b = *reinterpret_cast<const u32x4_a4*>(p + 4);
-    } else {
-      a = b = u32x4{0, 0, 0, 0};
+  __device__ __forceinline__ void load(const float* p) {
+    a = *reinterpret_cast<const u32x4_a4*>(p);
+    b = *reinterpret_cast<const u32x4_a4*>(p + 4);
+  }
+  __device__ __forceinline__ void load_some(const float* p, int nv) {
+    a = b = u32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < 7; ++j)
-        if (j < nv) {
-          const uint32_t w = __builtin_bit_cast(uint32_t, p[j]);
-          if (j < 4) a[j & 3] = w;
-          else b[j & 3] = w;
-        }
-    }
+    for (int j = 0; j < 8; ++j)
+      if (j < nv) {
+        const uint32_t w = __builtin_bit_cast(uint32_t, p[j]);
+        if (j < 4) a[j & 3] = w;
+        else b[j & 3] = w;
+      }
+  }
+  __device__ __forceinline__ void cut(int s) {
+    if (s == 0) return;
+    if (s & 4) { a = b; b = u32x4{0, 0, 0, 0}; }
+    if (s & 2) { a = u32x4{a[2], a[3], b[0], b[1]}; b = u32x4{b[2], b[3], 0, 0}; }
+    if (s & 1) { a = u32x4{a[1], a[2], a[3], b[0]}; b = u32x4{b[1], b[2], b[3], 0}; }
+    if (s & 8) a = b = u32x4{0, 0, 0, 0};
   }
   __device__ __forceinline__ void store(float* p, int nv) const {
     if (nv >= 8) {
       *reinterpret_cast<u32x4_a4*>(p) = a;
       *reinterpret_cast<u32x4_a4*>(p + 4) = b;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 7; ++j)
-        if (j < nv) p[j] = __builtin_bit_cast(float, j < 4 ? a[j & 3] : b[j & 3]);
+      return;
     }
+    if (nv & 4) *reinterpret_cast<u32x4_a4*>(p) = a;
+    const u32x4 t = (nv & 4) ? b : a;
+    p += nv & 4;
+    if (nv & 2) *reinterpret_cast<u32x2_a4*>(p) = u32x2{t[0], t[1]};
+    if (nv & 1) p[nv & 2] = __builtin_bit_cast(float, (nv & 2) ? (uint32_t)t[2] : (uint32_t)t[0]);
   }
   __device__ __forceinline__ float get(int j) const { return __builtin_bit_cast(float, j < 4 ? a[j & 3] : b[j & 3]); }
   __device__ __forceinline__ void set(const float (&v)[8]) {
@@ -124,29 +177,35 @@ template <> struct Vec8<float> {
 };
 struct Vec8Half {       // f16 and bf16: eight elements in four words
   u32x4 a;
-  __device__ __forceinline__ void load(const uint16_t* p, int nv) {
-    if (nv >= 8) {
-      a = *reinterpret_cast<const u32x4_a2*>(p);
-    } else {
-      a = u32x4{0, 0, 0, 0};
+  __device__ __forceinline__ void load(const void* p) { a = *reinterpret_cast<const u32x4_a2*>(p); }
+  __device__ __forceinline__ void load_some(const void* q, int nv) {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(q);
+    a = u32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < 7; ++j)
-        if (j < nv) a[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
-    }
+    for (int j = 0; j < 8; ++j)
+      if (j < nv) a[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
   }
-  __device__ __forceinline__ void store(uint16_t* p, int nv) const {
+  __device__ __forceinline__ void cut(int s) {
+    if (s == 0) return;
+    if (s & 4) a = u32x4{a[2], a[3], 0, 0};
+    if (s & 2) a = u32x4{a[1], a[2], a[3], 0};
+    if (s & 1) a = u32x4{a[0] >> 16 | a[1] << 16, a[1] >> 16 | a[2] << 16, a[2] >> 16 | a[3] << 16, a[3] >> 16};
+    if (s & 8) a = u32x4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ void store(void* q, int nv) const {
+    uint16_t* p = reinterpret_cast<uint16_t*>(q);
     if (nv >= 8) {
       *reinterpret_cast<u32x4_a2*>(p) = a;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 7; ++j)
-        if (j < nv) p[j] = (uint16_t)(a[j >> 1] >> (16 * (j & 1)));
+      return;
     }
+    if (nv & 4) *reinterpret_cast<u32x2_a2*>(p) = u32x2{a[0], a[1]};
+    const u32x2 t = (nv & 4) ? u32x2{a[2], a[3]} : u32x2{a[0], a[1]};
+    p += nv & 4;
+    if (nv & 2) *reinterpret_cast<u32_a2*>(p) = t[0];
+    if (nv & 1) p[nv & 2] = (uint16_t)((nv & 2) ? t[1] : t[0]);
   }
 };
 template <> struct Vec8<_Float16> : Vec8Half {
-  __device__ __forceinline__ void load(const _Float16* p, int nv) { Vec8Half::load(reinterpret_cast<const uint16_t*>(p), nv); }
-  __device__ __forceinline__ void store(_Float16* p, int nv) const { Vec8Half::store(reinterpret_cast<uint16_t*>(p), nv); }
   __device__ __forceinline__ float get(int j) const {
     const uint32_t w = a[j >> 1];      // a copy: __builtin_bit_cast of a vector's element to a vector reads the vector's first word
     return (float)__builtin_bit_cast(f16x2, w)[j & 1];
@@ -157,10 +216,9 @@ template <> struct Vec8<_Float16> : Vec8Half {
   }
 };
 template <> struct Vec8<__bf16> : Vec8Half {
-  __device__ __forceinline__ void load(const __bf16* p, int nv) { Vec8Half::load(reinterpret_cast<const uint16_t*>(p), nv); }
-  __device__ __forceinline__ void store(__bf16* p, int nv) const { Vec8Half::store(reinterpret_cast<uint16_t*>(p), nv); }
   __device__ __forceinline__ float get(int j) const {
-    return __builtin_bit_cast(float, (j & 1) ? a[j >> 1] & 0xffff0000u : a[j >> 1] << 16);
+    const uint32_t w = a[j >> 1];
+    return __builtin_bit_cast(float, (j & 1) ? w & 0xffff0000u : w << 16);
   }
   __device__ __forceinline__ void set(const float (&v)[8]) {     // v_cvt_pk_bf16_f32: nearest even
 #pragma unroll
@@ -195,26 +253,6 @@ int norm_forward(const NormArgs& a, hipStream_t stream);
 int norm_backward(const NormArgs& a, hipStream_t stream);
 uint64_t norm_workspace_bytes(long long rows, long long cols);
 int dropout(const void* x, void* y, long long n, int type, const DropArgs& d, hipStream_t stream);
-
-// weight / bias as fp32 (absent: `dflt`)
-template <class TX> __device__ __forceinline__ void load_param(const void* p, int p_f32, long long c, int nv, float dflt, float (&v)[8]) {
-  if (p == nullptr) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = dflt;
-    return;
-  }
-  if (p_f32) {
-    Vec8<float> r;
-    r.load(reinterpret_cast<const float*>(p) + c, nv);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = r.get(j);
-  } else {
-    Vec8<TX> r;
-    r.load(reinterpret_cast<const TX*>(p) + c, nv);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = r.get(j);
-  }
-}
 
 // z = residual + dropout(x) for eight elements, the same expression in both passes.  A dropped element counts as zero whatever its
 // value (a NaN or infinity that is dropped leaves no trace).

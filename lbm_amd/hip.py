@@ -569,7 +569,7 @@ def _as_rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
         rows = [(s, d) for s, d in zip(shape[:-1], stride[:-1]) if s != 1]
         if all(rows[i][1] == rows[i + 1][1] * rows[i + 1][0] for i in range(len(rows) - 1)):
             ld = rows[-1][1] if rows else n
-            if ld >= n:
+            if n <= ld < 1 << 31:
                 return t, ld
     return t.contiguous(), n
 
