@@ -23,10 +23,10 @@ struct NormShape {
   bool block;       // a team is a workgroup
   int teams() const { return block ? 1 : threads >> shift; }
 };
-inline NormShape norm_shape(long long cols) {
+inline NormShape norm_shape(long long cols, int most) {        // most: chunks that a wave may hold
   NormShape s{1, 0, 256, false};
   const int chunks = (int)((cols + 7) / 8);
-  if (chunks > 256) {
+  if (chunks > most) {
     s.block = true;
     s.k = 2;
     s.threads = (chunks + 127) / 128 * 64;
@@ -100,6 +100,50 @@ __device__ __forceinline__ float lanes_sum(float v, int shift) {
   return v;
 }
 __device__ __forceinline__ float wave64_sum(float v) { return lane32_sum(lane16_sum(row16_sum(v))); }
+
+__device__ __forceinline__ u32x4 from_lane(const u32x4& v, int lane) {
+  return u32x4{(uint32_t)__shfl((int)v[0], lane), (uint32_t)__shfl((int)v[1], lane), (uint32_t)__shfl((int)v[2], lane), (uint32_t)__shfl((int)v[3], lane)};
+}
+// The masks of a thread's K chunks; e0: the row's first element.  In a row whose length is no multiple of eight a chunk lies in two blocks,
+// the second of which is the next chunk's first: it is fetched from the lane that drew it, and only behind a stripe's last lane one
+// more is drawn.  BLK: a stripe (chunks k * lanes ...) runs over several waves, and lane k draws what lane 63 lacks of stripe k.
+template <int K, bool BLK>
+__device__ __forceinline__ void keep_row(Keep8 (&m)[K], uint64_t e0, const DropKey& key, uint32_t tm1, int cols, int lanes, int tl) {
+  u32x4 w[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) w[k] = philox(2 * ((e0 >> 3) + (uint32_t)(k * lanes + tl)), key);
+  if ((cols & 7) != 0) {
+    const uint32_t sh = (uint32_t)e0 & 7u;
+    const int seg = BLK ? 64 : lanes, self = threadIdx.x & 63, pos = self & (seg - 1), base = self - pos;
+    u32x4 next[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) next[k] = from_lane(w[k], base + ((pos + 1) & (seg - 1)));
+    if (BLK) {
+      const u32x4 extra = philox(2 * ((e0 >> 3) + (uint32_t)((pos & 3) * lanes + tl - pos + 64)), key);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const u32x4 v = from_lane(extra, k);
+        if (pos == 63) next[k] = v;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k + 1 < K; ++k) {
+        const u32x4 v = from_lane(w[k + 1], base);
+        if (pos == lanes - 1) next[k] = v;
+      }
+      if (cols > (K * lanes - 1) * 8) {                    // the last lane's last chunk exists
+        const u32x4 extra = philox(2 * ((e0 >> 3) + (uint32_t)(K * lanes)), key);
+        if (pos == lanes - 1) next[K - 1] = extra;
+      }
+    }
+    if (sh != 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) w[k] = straddle(w[k], next[k], sh);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) m[k] = keep_from(w[k], e0 + (uint32_t)((k * lanes + tl) * 8), key, tm1);
+}
 
 // calls f<TX, TR, RES>(a, s) for the types of a
 #define NORM_DISPATCH(F, a, s)                                                                            \

@@ -4,13 +4,11 @@
 // A team of threads (norm.hpp) holds a row in registers; a thread owns the same columns of every row that its team works on, so the sums
 // over rows are private registers until the workgroup's teams are added up through LDS and written as one partial sum
 // [2][cols] a workgroup.  norm_finish adds the partial sums in a fixed order: no atomics, the same bits every time.
+#include <algorithm>
+
 #include "norm.hpp"
 
 namespace lbm {
-
-#ifndef NB_G
-#define NB_G 512
-#endif
 
 // dweight / dbias from the first partial sum when it is the only one
 template <class T> __device__ __forceinline__ void put_sum(const NormArgs& a, int which, long long c, float v) {
@@ -33,18 +31,18 @@ template <class TX, class TR, int K> struct BwdRow {
 // One row of a team: xhat and g = dy w from what was loaded, their two sums (s1 = sum g, s2 = sum g xhat), the columns' sums.
 // w: this thread's weights, from LDS where K > 1 (their registers would cost a wave a SIMD; a fetch is two ds_read_b128 a chunk).
 // gone: a row past the last one, of which nothing counts.
-template <class TX, class TR, int RES, int K>
+template <class TX, class TR, int RES, int K, bool BLK>
 __device__ __forceinline__ void bwd_row(const NormArgs& a, const DropKey& key, BwdRow<TX, TR, K>& in, const Span (&sp)[K], bool gone, long long row,
                                         int lanes, int tl, const float* w, float (&xh)[K][8], float (&g)[K][8], Keep8 (&m)[K],
                                         float (&dw)[K][8], float (&db)[K][8], float& s1, float& s2) {
   s1 = s2 = 0.0f;
+  if (RES && a.drop.on) keep_row<K, BLK>(m, (uint64_t)(row * a.cols), key, a.drop.tm1, (int)a.cols, lanes, tl);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     in.x[k].cut(sp[k].cut);
     in.d[k].cut(gone ? 8 : sp[k].cut);
     if (RES) in.r[k].cut(sp[k].cut);
     if (RES && a.drop.on) {
-      m[k] = keep8((uint64_t)(row * a.cols + (k * lanes + tl) * 8), key, a.drop.tm1);
       const uint32_t limit = keep_limit(a.drop.tm1);
 #pragma unroll
       for (int j = 0; j < 8; ++j) xh[k][j] = join_one<RES>(in.x[k].get(j), in.r[k].get(j), m[k].kept(j, limit), a.drop.scale);
@@ -143,7 +141,7 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a, int shift) {
     float xh[K][8], g[K][8], s1, s2;
     Keep8 m[K];
     const float rstd = in.rstd;
-    bwd_row<TX, TR, RES, K>(a, key, in, sp, row >= a.rows, row, lanes, tl, K > 1 ? red : w, xh, g, m, dw, db, s1, s2);
+    bwd_row<TX, TR, RES, K, false>(a, key, in, sp, row >= a.rows, row, lanes, tl, K > 1 ? red : w, xh, g, m, dw, db, s1, s2);
     if (base + step < a.rows) load(base + step);
     const float c1 = lanes_sum(s1, shift) * inv, c2 = lanes_sum(s2, shift) * inv;
     if (row < a.rows) bwd_put<TX, TR, RES, K>(a, sp, row * a.cols, lanes, tl, c1, c2, rstd, xh, g, m);
@@ -212,7 +210,7 @@ __global__ __launch_bounds__(AHEAD ? 512 : 1024) void norm_bwd_block_kernel(Norm
     float xh[K][8], g[K][8], s1, s2;
     Keep8 m[K];
     const float rstd = in.rstd;
-    bwd_row<TX, TR, RES, K>(a, key, in, sp, false, row, lanes, tl, wlds, xh, g, m, dw, db, s1, s2);
+    bwd_row<TX, TR, RES, K, true>(a, key, in, sp, false, row, lanes, tl, wlds, xh, g, m, dw, db, s1, s2);
     if (AHEAD && row + gridDim.x < a.rows) load(row + gridDim.x);
     // one barrier a row: the next row writes the other half, and the one after it finds every thread past this row's reads
     s1 = wave64_sum(s1);
@@ -273,32 +271,35 @@ int norm_finish(const NormArgs& a, int parts, hipStream_t s) {
 }
 
 // The teams of the backward pass: more than 1024 columns belong to a workgroup (K = 4 in a wave leaves one wave a SIMD), more than 4096 to
-// K = 4 chunks a thread where those and the loads ahead fit 256 registers: half precision without a residual.
+// K = 4 chunks a thread where those and the loads ahead fit 256 registers (lean: half precision without a residual).
 static NormShape bwd_shape(long long cols, bool lean) {
   const int chunks = (int)((cols + 7) / 8);
-  if (chunks <= 128) return norm_shape(cols);
+  if (chunks <= 128) return norm_shape(cols, 128);
   NormShape s{chunks > 512 && lean ? 4 : 2, 0, 0, true};
   s.threads = (chunks + 64 * s.k - 1) / (64 * s.k) * 64;
   return s;
 }
-// workgroups = partial sums; no type changes their number
-static int norm_parts(long long rows, long long cols) {
-  const NormShape sh = bwd_shape(cols, false);
+// workgroups = partial sums: what is resident at once, a whole number a CU (the sums a workgroup keeps make the launch persistent)
+static int norm_parts(long long rows, long long cols, bool lean) {
+  const NormShape sh = bwd_shape(cols, lean);
+  int per_cu = 2;
+  if (sh.block) per_cu = sh.k == 4 ? 1 : sh.threads <= 128 ? 3 : sh.threads <= 256 ? 2 : 1024 / sh.threads;
+  while (sh.block && per_cu > 1 && rows < 8 * 256 * per_cu) --per_cu;      // a partial sum costs as much traffic as four rows
   const long long g = (rows + sh.teams() - 1) / sh.teams();
-  const long long most = !sh.block ? NB_G : 256 * (sh.threads <= 128 ? 3 : sh.threads <= 256 ? 2 : 1);
-  return (int)(g < 1 ? 1 : g < most ? g : most);
+  return (int)(g < 1 ? 1 : g < 256 * per_cu ? g : 256 * per_cu);
 }
 
 uint64_t norm_workspace_bytes(long long rows, long long cols) {
-  const int parts = cols < kNormRowMin || cols > kNormRowMax ? norm_wide_parts(rows, cols) : norm_parts(rows, cols);
+  const int parts = cols < kNormRowMin || cols > kNormRowMax ? norm_wide_parts(rows, cols) : std::max(norm_parts(rows, cols, false), norm_parts(rows, cols, true));
   return (uint64_t)parts * 2 * (uint64_t)cols * sizeof(float);
 }
 
 template <class TX, class TR, int RES> static int backward(const NormArgs& a, hipStream_t s) {
-  const NormShape sh = bwd_shape(a.cols, RES == 0 && sizeof(TX) == 2);
-  const int grid = norm_parts(a.rows, a.cols);
+  constexpr bool lean = RES == 0 && sizeof(TX) == 2;
+  const NormShape sh = bwd_shape(a.cols, lean);
+  const int grid = norm_parts(a.rows, a.cols, lean);
   const size_t lds = (size_t)sh.threads * sh.k * 8 * sizeof(float);
-  if (sh.block && sh.k == 4) norm_bwd_block_kernel<TX, TR, RES, RES == 0 && sizeof(TX) == 2 ? 4 : 2, true><<<grid, sh.threads, lds, s>>>(a);
+  if (sh.block && sh.k == 4) norm_bwd_block_kernel<TX, TR, RES, lean ? 4 : 2, true><<<grid, sh.threads, lds, s>>>(a);
   else if (sh.block && sh.threads <= 256) norm_bwd_block_kernel<TX, TR, RES, 2, true><<<grid, sh.threads, lds, s>>>(a);
   else if (sh.block) norm_bwd_block_kernel<TX, TR, RES, 2, false><<<grid, sh.threads, lds, s>>>(a);
   else if (sh.k == 1) norm_bwd_kernel<TX, TR, RES, 1><<<grid, 256, 0, s>>>(a, sh.shift);

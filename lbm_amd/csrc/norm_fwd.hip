@@ -11,19 +11,20 @@ template <class TX, class TR, int K> struct FwdRow {
 };
 
 // z of a loaded row, its sum in s
-template <class TX, class TR, int RES, int K>
+template <class TX, class TR, int RES, int K, bool BLK>
 __device__ __forceinline__ float join_row(const NormArgs& a, const DropKey& key, FwdRow<TX, TR, K>& in, const Span (&sp)[K], long long row,
                                           int lanes, int tl, float (&z)[K][8]) {
   float s = 0.0f;
+  Keep8 m[K];
+  if (RES && a.drop.on) keep_row<K, BLK>(m, (uint64_t)(row * a.cols), key, a.drop.tm1, (int)a.cols, lanes, tl);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     in.x[k].cut(sp[k].cut);
     if (RES) in.r[k].cut(sp[k].cut);
     if (RES && a.drop.on) {
-      const Keep8 m = keep8((uint64_t)(row * a.cols + (k * lanes + tl) * 8), key, a.drop.tm1);
       const uint32_t limit = keep_limit(a.drop.tm1);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) z[k][j] = join_one<RES>(in.x[k].get(j), in.r[k].get(j), m.kept(j, limit), a.drop.scale);
+      for (int j = 0; j < 8; ++j) z[k][j] = join_one<RES>(in.x[k].get(j), in.r[k].get(j), m[k].kept(j, limit), a.drop.scale);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) z[k][j] = join_one<RES>(in.x[k].get(j), RES ? in.r[k].get(j) : 0.0f, true, 1.0f);
@@ -93,7 +94,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift) {
   for (int u = 0; u < U; ++u) {
     const int r = u * teams + team;
     float z[K][8];
-    const float mean = lanes_sum(join_row<TX, TR, RES, K>(a, key, in[u], sp, base + r, lanes, tl, z), shift) * inv;
+    const float mean = lanes_sum(join_row<TX, TR, RES, K, false>(a, key, in[u], sp, base + r, lanes, tl, z), shift) * inv;
     const float rstd = rsqrt_newton(lanes_sum(deviate<K>(z, mean, sp), shift) * inv + a.eps);
     if (r > last) continue;
     if (tl == 0 && a.mean != nullptr) {
@@ -137,7 +138,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
   }
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     float z[K][8];
-    const float s = join_row<TX, TR, RES, K>(a, key, in, sp, row, lanes, tl, z);
+    const float s = join_row<TX, TR, RES, K, true>(a, key, in, sp, row, lanes, tl, z);
     if (row + gridDim.x < a.rows) load(row + gridDim.x);
     const float mean = block_sum(s, sm[0]) * inv;
     const float rstd = rsqrt_newton(block_sum(deviate<K>(z, mean, sp), sm[1]) * inv + a.eps);
@@ -152,9 +153,9 @@ __global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
   }
 }
 
-#ifndef NF_GB
-#define NF_GB 512
+#ifndef NF_MANY
 #define NF_MANY 2048
+#define NF_JOIN 128
 #endif
 template <class TX, class TR, int RES, int K, int U> static int wave_forward(const NormArgs& a, const NormShape& sh, hipStream_t s) {
   const long long per = (long long)sh.teams() * U, grid = (a.rows + per - 1) / per;
@@ -163,9 +164,9 @@ template <class TX, class TR, int RES, int K, int U> static int wave_forward(con
   return check_launch("norm_forward");
 }
 template <class TX, class TR, int RES> static int forward(const NormArgs& a, hipStream_t s) {
-  const NormShape sh = norm_shape(a.cols);
+  const NormShape sh = norm_shape(a.cols, RES ? NF_JOIN : 256);
   if (sh.block) {
-    const long long most = NF_GB * 512 / sh.threads;
+    const long long most = 256 * (1024 / sh.threads);      // what is resident at once (16 waves a CU), a whole number a CU
     norm_fwd_block_kernel<TX, TR, RES, 2><<<(unsigned)(a.rows < most ? a.rows : most), sh.threads, 0, s>>>(a);
     return check_launch("norm_forward");
   }

@@ -99,18 +99,24 @@ __device__ __forceinline__ u32x4 straddle(const u32x4& a, const u32x4& b, uint32
   if (sh & 1) p = u32x4{p[0] >> 16 | p[1] << 16, p[1] >> 16 | p[2] << 16, p[2] >> 16 | p[3] << 16, p[3] >> 16 | q[0] << 16};
   return p;
 }
-// the eight elements from e on; rows whose length is no multiple of eight start anywhere in a block
-__device__ __forceinline__ Keep8 keep8(uint64_t e, const DropKey& k, uint32_t tm1) {
-  const uint32_t sh = (uint32_t)e & 7u;
-  const uint64_t b = e >> 3;
-  Keep8 m{philox(2 * b, k)};
-  if (sh != 0) m.w = straddle(m.w, philox(2 * b + 2, k), sh);
+// the eight elements from e on, `high` being the numbers' upper halves; rows whose length is no multiple of eight start anywhere in a block
+__device__ __forceinline__ Keep8 keep_from(u32x4 high, uint64_t e, const DropKey& k, uint32_t tm1) {
+  Keep8 m{high};
   if (any_tie(m.w, tm1)) {
+    const uint32_t sh = (uint32_t)e & 7u;
+    const uint64_t b = e >> 3;
     u32x4 low = philox(2 * b + 1, k);
     if (sh != 0) low = straddle(low, philox(2 * b + 3, k), sh);
     settle_ties(m.w, low, tm1);
   }
   return m;
+}
+__device__ __forceinline__ Keep8 keep8(uint64_t e, const DropKey& k, uint32_t tm1) {
+  const uint32_t sh = (uint32_t)e & 7u;
+  const uint64_t b = e >> 3;
+  u32x4 high = philox(2 * b, k);
+  if (sh != 0) high = straddle(high, philox(2 * b + 2, k), sh);
+  return keep_from(high, e, k, tm1);
 }
 
 // ---- eight consecutive elements of a row ---------------------------------------------------------------------------
