@@ -28,5 +28,5 @@ def __getattr__(name):
         return MultiScaleDeformableAttention
     if name in ("layer_norm", "dropout", "dropout_add_layer_norm"):
         from . import training
-        return getattr(training, name)
+        return globals().setdefault(name, getattr(training, name))
     raise AttributeError(name)

@@ -286,7 +286,8 @@ static int norm_parts(long long rows, long long cols, bool lean) {
   if (sh.block) per_cu = sh.k == 4 ? 1 : sh.threads <= 128 ? 3 : sh.threads <= 256 ? 2 : 1024 / sh.threads;
   while (sh.block && per_cu > 1 && rows < 8 * 256 * per_cu) --per_cu;      // a partial sum costs as much traffic as four rows
   const long long g = (rows + sh.teams() - 1) / sh.teams();
-  return (int)(g < 1 ? 1 : g < 256 * per_cu ? g : 256 * per_cu);
+  if (g <= 8) return 1;                    // a few rounds of one workgroup cost less than the second launch
+  return (int)std::min(g, 256ll * per_cu);
 }
 
 uint64_t norm_workspace_bytes(long long rows, long long cols) {

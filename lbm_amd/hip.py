@@ -545,119 +545,50 @@ def l2norm(x: torch.Tensor) -> torch.Tensor:
     return y
 
 
-# ---- training operators (differentiable forms: lbm_amd/training.py) ----
+# ---- training operators: one pass each (differentiable: lbm_amd/training.py; both call the host path in csrc/torch_ops.cpp) ----
 
-_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}       # LBM_TYPE_*
-
-
-def _elem_type(t: torch.Tensor, what: str) -> int:
-    if not t.is_cuda:
-        raise HipError(f"{what}: expected a GPU tensor")
-    code = _TYPES.get(t.dtype)
-    if code is None:
-        raise HipError(f"{what}: expected float32, float16 or bfloat16, got {t.dtype}")
-    return code
+_ops = None
 
 
-def _as_rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
-    """(t, elements between rows): rows of the last dimension at one stride are used where they lie, any other layout is copied."""
-    n = t.shape[-1]
-    if t.is_contiguous():
-        return t, n
-    shape, stride = t.shape, t.stride()
-    if stride[-1] == 1 and t.numel():
-        rows = [(s, d) for s, d in zip(shape[:-1], stride[:-1]) if s != 1]
-        if all(rows[i][1] == rows[i + 1][1] * rows[i + 1][0] for i in range(len(rows) - 1)):
-            ld = rows[-1][1] if rows else n
-            if n <= ld < 1 << 31:
-                return t, ld
-    return t.contiguous(), n
+def ops():
+    """lbm_amd/_torch_ops.so bound to the loaded library's entry points; raises if it has not been built."""
+    global _ops
+    if _ops is None:
+        lib = load()
+        try:
+            from . import _torch_ops as m
+        except ImportError as e:
+            raise HipError(f"lbm_amd/_torch_ops.so cannot be loaded ({e}): build it with `make -C {_HERE / 'csrc'}`") from e
+        m.bind(*(C.cast(getattr(lib, "lbm_hip_" + n), C.c_void_p).value for n in
+                 ("norm_forward", "norm_backward", "dropout", "norm_workspace_bytes", "last_error")), HipError)
+        _ops = m
+    return _ops
 
 
-def _drop_args(p, seed, offset, device, what: str):
-    """-> (p, seed value, its device pointer, offset) of a dropout mask; seed: an integer or an int64 GPU tensor of one element."""
-    p, offset = float(p), operator.index(offset)
-    if not 0.0 <= p <= 1.0:
-        raise HipError(f"{what}: p = {p} is not a probability")
+def _drop_args(p, seed, offset):
+    """-> (p, seed, seed tensor or None, offset) of a dropout mask as the host path takes them."""
+    offset = operator.index(offset)
     if not 0 <= offset < 1 << 64:
-        raise HipError(f"{what}: offset {offset} is outside 0 .. 2^64 - 1")
+        raise HipError(f"offset {offset} is outside 0 .. 2^64 - 1")
     if isinstance(seed, torch.Tensor):
-        if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
-            raise HipError(f"{what}: a seed tensor holds one int64 on the operands' device")
-        return p, 0, seed.data_ptr(), offset
+        return p, 0, seed, offset
     seed = operator.index(seed)
     if not -(1 << 63) <= seed < 1 << 64:
-        raise HipError(f"{what}: seed {seed} does not fit 64 bits")
+        raise HipError(f"seed {seed} does not fit 64 bits")
     return p, seed & 0xFFFFFFFFFFFFFFFF, None, offset
-
-
-def _call_on(device: torch.device, fn, what: str, *args) -> None:
-    """fn(*args, stream) on the current stream of the operands' device, whichever device is the current one."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
-    if rc != 0:
-        _check(rc, what)
 
 
 def dropout(x: torch.Tensor, p: float, seed, offset: int = 0) -> torch.Tensor:
     """x / (1 - p) where the mask of (seed, offset) keeps an element, else 0 (lbm_hip_dropout); dense result.  On dy: the gradient."""
-    code = _elem_type(x, "dropout")
-    p, seed_value, seed_dev, offset = _drop_args(p, seed, offset, x.device, "dropout")
-    x = x.contiguous()
-    y = torch.empty_like(x)
-    _call_on(x.device, load().lbm_hip_dropout, "lbm_hip_dropout", x.data_ptr(), y.data_ptr(), x.numel(), code, p, seed_value, seed_dev, offset)
-    return y
-
-
-def _norm_operands(what: str, x, residual, weight, bias):
-    """Checks shared by both passes -> (x, ld_x, residual, ld_residual, weight, bias, x_type, res_type, param_type)."""
-    tx = tr = tp = _elem_type(x, what)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise HipError(f"{what}: x needs a last dimension of at least one element, got shape {tuple(x.shape)}")
-    dev, ldr = x.device, 0
-    x, ldx = _as_rows(x)
-    if residual is not None:
-        tr = _elem_type(residual, what)
-        if residual.shape != x.shape or residual.device != dev:
-            raise HipError(f"{what}: residual has shape {tuple(residual.shape)} on {residual.device}, x {tuple(x.shape)} on {dev}")
-        if tr != tx and tr != 0:
-            raise HipError(f"{what}: the residual's type must be x's ({x.dtype}) or float32, got {residual.dtype}")
-        residual, ldr = _as_rows(residual)
-    given = [t for t in (weight, bias) if t is not None]
-    for t in given:
-        tp = _elem_type(t, what)
-        if t.shape != x.shape[-1:] or t.device != dev:
-            raise HipError(f"{what}: weight / bias have shape {tuple(t.shape)} on {t.device}, expected ({x.shape[-1]},) on {dev}")
-        if tp != tx and tp != 0:
-            raise HipError(f"{what}: the type of weight and bias must be x's ({x.dtype}) or float32, got {t.dtype}")
-    if len(given) == 2 and weight.dtype != bias.dtype:
-        raise HipError(f"{what}: weight and bias differ in type ({weight.dtype}, {bias.dtype})")
-    return (x, ldx, residual, ldr, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), tx, tr, tp)
-
-
-def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+    return ops().dropout_pass(x, *_drop_args(p, seed, offset))
 
 
 def norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float = 1e-5,
                  residual: Optional[torch.Tensor] = None, p: float = 0.0, seed=0, offset: int = 0, want_stats: bool = False):
     """layer_norm of x, or of residual + dropout(x) (lbm_hip_norm_forward) -> y in the residual's type (x's without one), dense;
     with want_stats (y, mean, rstd): what norm_backward needs beside the inputs."""
-    x, ldx, residual, ldr, weight, bias, tx, tr, tp = _norm_operands("norm_forward", x, residual, weight, bias)
-    p, seed_value, seed_dev, offset = _drop_args(p, seed, offset, x.device, "norm_forward")
-    cols = x.shape[-1]
-    rows = x.numel() // cols
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype if residual is None else residual.dtype)
-    mean = rstd = None
-    if want_stats:
-        mean, rstd = torch.empty(2, rows, device=x.device, dtype=torch.float32).unbind(0)
-    d = NormDesc(x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(mean), _ptr(rstd), None, None, None, None, None,
-                 None, 0, rows, cols, ldx, ldr, 0, tx, tr, tp, eps, p, seed_value, offset, seed_dev)
-    _call_on(x.device, load().lbm_hip_norm_forward, "lbm_hip_norm_forward", C.byref(d))
-    return (y, mean, rstd) if want_stats else y
+    y, st = ops().norm_forward(x, residual, weight, bias, eps, *_drop_args(p, seed, offset), want_stats)
+    return (y, st[0], st[1]) if want_stats else y
 
 
 def norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: Optional[torch.Tensor],
@@ -665,29 +596,7 @@ def norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: t
                   offset: int = 0, want: Sequence[bool] = (True, True, True, True)):
     """Gradients of norm_forward at dy (lbm_hip_norm_backward) -> (dx, dresidual, dweight, dbias), None where `want` is false or the
     operand is absent.  The arguments are the forward call's; mean and rstd its statistics."""
-    x, ldx, residual, ldr, weight, bias, tx, tr, tp = _norm_operands("norm_backward", x, residual, weight, bias)
-    p, seed_value, seed_dev, offset = _drop_args(p, seed, offset, x.device, "norm_backward")
-    dev, cols = x.device, x.shape[-1]
-    rows = x.numel() // cols
-    ytype = x.dtype if residual is None else residual.dtype
-    if dy.shape != x.shape or dy.dtype != ytype or dy.device != dev:
-        raise HipError(f"norm_backward: dy has shape {tuple(dy.shape)}, type {dy.dtype}, on {dy.device}; expected {tuple(x.shape)}, {ytype}, on {dev}")
-    for t in (mean, rstd):
-        if t.dtype != torch.float32 or t.numel() != rows or t.device != dev or not t.is_contiguous():
-            raise HipError("norm_backward: mean and rstd are the dense fp32 statistics of norm_forward, one a row")
-    dy, lddy = _as_rows(dy)
-    dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if want[0] else None
-    dres = torch.empty(x.shape, device=dev, dtype=ytype) if want[1] and residual is not None else None
-    dw = torch.empty_like(weight) if want[2] and weight is not None else None
-    db = torch.empty_like(bias) if want[3] and bias is not None else None
-    lib, ws, nbytes = load(), None, 0
-    if dw is not None or db is not None:
-        nbytes = lib.lbm_hip_norm_workspace_bytes(rows, cols)
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    d = NormDesc(x.data_ptr(), _ptr(residual), _ptr(weight), _ptr(bias), None, mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), _ptr(dx),
-                 _ptr(dres), _ptr(dw), _ptr(db), _ptr(ws), nbytes, rows, cols, ldx, ldr, lddy, tx, tr, tp, eps, p, seed_value, offset, seed_dev)
-    _call_on(dev, lib.lbm_hip_norm_backward, "lbm_hip_norm_backward", C.byref(d))
-    return dx, dres, dw, db
+    return tuple(ops().norm_backward(dy, x, mean, rstd, residual, weight, bias, eps, *_drop_args(p, seed, offset), *want))
 
 
 def attn_readout(U, seq, S, ring_head=0, temb=None, mask_a=None, mask_b=None, want_valid=False):
