@@ -270,12 +270,13 @@ int norm_finish(const NormArgs& a, int parts, hipStream_t s) {
   return check_launch("norm_backward");
 }
 
-// The teams of the backward pass: more than 1024 columns belong to a workgroup (K = 4 in a wave leaves one wave a SIMD), more than 4096 to
-// K = 4 chunks a thread where those and the loads ahead fit 256 registers (lean: half precision without a residual).
+// The teams of the backward pass: more than 1024 columns belong to a workgroup (K = 4 in a wave leaves one wave a SIMD).  Up to 8192 columns
+// it has 512 threads at most, with registers for the loads ahead; beyond, K = 4 chunks a thread where they fit beside those (lean: half
+// precision without a residual), else 1024 threads that load a row at a time.
 static NormShape bwd_shape(long long cols, bool lean) {
   const int chunks = (int)((cols + 7) / 8);
   if (chunks <= 128) return norm_shape(cols, 128);
-  NormShape s{chunks > 512 && lean ? 4 : 2, 0, 0, true};
+  NormShape s{chunks > 1024 && lean ? 4 : 2, 0, 0, true};
   s.threads = (chunks + 64 * s.k - 1) / (64 * s.k) * 64;
   return s;
 }
@@ -283,7 +284,7 @@ static NormShape bwd_shape(long long cols, bool lean) {
 static int norm_parts(long long rows, long long cols, bool lean) {
   const NormShape sh = bwd_shape(cols, lean);
   int per_cu = 2;
-  if (sh.block) per_cu = sh.k == 4 ? 1 : sh.threads <= 128 ? 3 : sh.threads <= 256 ? 2 : 1024 / sh.threads;
+  if (sh.block) per_cu = sh.threads <= 128 ? 3 : sh.threads <= 256 ? 2 : 1;
   while (sh.block && per_cu > 1 && rows < 8 * 256 * per_cu) --per_cu;      // a partial sum costs as much traffic as four rows
   const long long g = (rows + sh.teams() - 1) / sh.teams();
   if (g <= 8) return 1;                    // a few rounds of one workgroup cost less than the second launch
@@ -301,7 +302,7 @@ template <class TX, class TR, int RES> static int backward(const NormArgs& a, hi
   const int grid = norm_parts(a.rows, a.cols, lean);
   const size_t lds = (size_t)sh.threads * sh.k * 8 * sizeof(float);
   if (sh.block && sh.k == 4) norm_bwd_block_kernel<TX, TR, RES, lean ? 4 : 2, true><<<grid, sh.threads, lds, s>>>(a);
-  else if (sh.block && sh.threads <= 256) norm_bwd_block_kernel<TX, TR, RES, 2, true><<<grid, sh.threads, lds, s>>>(a);
+  else if (sh.block && sh.threads <= 512) norm_bwd_block_kernel<TX, TR, RES, 2, true><<<grid, sh.threads, lds, s>>>(a);
   else if (sh.block) norm_bwd_block_kernel<TX, TR, RES, 2, false><<<grid, sh.threads, lds, s>>>(a);
   else if (sh.k == 1) norm_bwd_kernel<TX, TR, RES, 1><<<grid, 256, 0, s>>>(a, sh.shift);
   else if (sh.k == 2) norm_bwd_kernel<TX, TR, RES, 2><<<grid, 256, 0, s>>>(a, sh.shift);
