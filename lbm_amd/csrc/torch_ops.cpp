@@ -2,6 +2,7 @@
 // lbm_hip_norm_backward and lbm_hip_dropout.  A training step of the tracker's sizes calls them for a few microseconds of GPU work each,
 // forty times a step: the same path in Python took 16 us a forward and, in the thread that autograd runs a GPU's nodes in, 35 us a
 // backward call.  No kernels here; the entry points come as addresses from the library that lbm_amd/hip.py has loaded.
+#include <initializer_list>
 #include <mutex>
 #include <optional>
 #include <string>
@@ -9,6 +10,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
@@ -49,6 +51,7 @@ std::string text(const Tensor& t) {
 }
 
 int elem_type(const Tensor& t, const char* what) {
+  TORCH_CHECK(api.forward != nullptr, "lbm_amd._torch_ops is used through lbm_amd.hip.ops()");
   if (!t.is_cuda()) fail(std::string(what) + ": expected a GPU tensor, got " + text(t));
   switch (t.scalar_type()) {
     case at::kFloat: return LBM_TYPE_F32;
@@ -286,9 +289,29 @@ struct DropoutBackward : public Node {
 
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// What a graph of these operators would get wrong without an error: forward-mode derivatives, which they do not carry on; and a step
+// captured while an eager graph on the default stream still holds the leaves -- the backward pass would make that stream wait
+// inside the capture, which the default stream cannot.
+void refuse(const char* what, std::initializer_list<const Tensor*> inputs, bool grad) {
+  for (const Tensor* t : inputs)
+    if (t->defined() && t->_fw_grad(0).defined()) fail(std::string(what) + ": forward-mode derivatives are not supported");
+  // (the default stream cannot capture, and asking it while another stream does is an error)
+  if (!grad || c10::hip::getCurrentHIPStream().id() == 0 || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const Tensor* t : inputs) {
+    if (!wants_grad(*t) || !t->is_leaf()) continue;
+    const auto leaf = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!leaf) continue;
+    const auto stream = leaf->stream();
+    if (stream.has_value() && stream->id() == 0)
+      fail(std::string(what) + ": captured while an eager graph on the default stream still holds the leaf " + text(*t) + ": release that graph first");
+  }
+}
+
 Tensor dropout(const Tensor& x, const Drop& drop) {
   std::shared_ptr<DropoutBackward> node;
-  if (c10::GradMode::is_enabled() && wants_grad(x)) {
+  const bool grad = c10::GradMode::is_enabled() && wants_grad(x);
+  refuse("dropout", {&x}, grad);
+  if (grad) {
     node = std::shared_ptr<DropoutBackward>(new DropoutBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(x));
     node->seed = saved(drop.seed_dev);
@@ -306,6 +329,7 @@ Tensor dropout(const Tensor& x, const Drop& drop) {
 
 Tensor norm(const char* what, const Tensor& x, const Tensor& residual, const Tensor& weight, const Tensor& bias, double eps, const Drop& drop) {
   const bool grad = c10::GradMode::is_enabled() && (wants_grad(x) || wants_grad(residual) || wants_grad(weight) || wants_grad(bias));
+  refuse(what, {&x, &residual, &weight, &bias}, grad);
   std::tuple<Tensor, Tensor> r;
   Operands o;
   {

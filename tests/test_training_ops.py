@@ -556,6 +556,130 @@ def test_captured_autograd_step():
 
 
 @gpu
+def test_capture_beside_a_living_eager_graph_is_refused():
+    """An eager graph on the default stream holds the leaf's gradient node: a captured backward pass would wait on the default stream."""
+    w = torch.ones(32, device="cuda").requires_grad_()
+    x = torch.randn(4, 32, device="cuda")
+    alive = layer_norm(x, w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    out = None
+    with torch.cuda.graph(graph):
+        out = x + 1
+        with pytest.raises(hip.HipError, match="eager graph"):
+            layer_norm(x, w)
+    del alive
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer_norm(x, w).detach()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, layer_norm(x, w.detach()))
+
+
+@gpu
+def test_x_is_its_own_residual():
+    o = operands((20, 48), F32, F32, F32, "both", seed=21)
+    x = o["x"].clone().requires_grad_()
+    dropout_add_layer_norm(x, x, o["weight"], o["bias"], p=0.5, seed=2, offset=3).backward(o["dy"])
+    factor = ref.keep((20, 48), 0.5, 2, 3).double() * ref.scale(0.5)
+    want = ref.norm(o["x"], o["weight"], o["bias"], 1e-5, o["x"], factor, o["dy"])
+    tol = bounds(want, 1e-5, F32, F32, F32, 2.0)
+    within(x.grad, want["dx"] + want["dresidual"], tol["dx"] + tol["dresidual"] + u(F32) * (want["dx"] + want["dresidual"]).abs(), "dx")
+
+
+@gpu
+def test_backward_again():
+    o = operands((20, 48), F32, F32, F32, "both", seed=22)
+    x = o["x"].clone().requires_grad_()
+    y = dropout_add_layer_norm(x, o["residual"], o["weight"], o["bias"], p=0.5, seed=2)
+    a, = torch.autograd.grad(y, x, o["dy"], retain_graph=True)
+    b, = torch.autograd.grad(y, x, o["dy"])
+    assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, x, o["dy"])
+
+
+@gpu
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpointed_block(reentrant):
+    """The mask is an argument's function, so a recomputed forward pass draws it again: the same bits as without a checkpoint."""
+    from torch.utils.checkpoint import checkpoint
+    o = operands((50, 256), F16, F32, F32, "both", seed=23)
+
+    def block(x, r, w, b):
+        return layer_norm(dropout_add_layer_norm(dropout(x, 0.2, 5, 1), r, w, b, p=0.3, seed=5, offset=2), w, b)
+
+    results = []
+    for how in ("plain", "checkpoint"):
+        t = [o[k].detach().clone().requires_grad_() for k in ("x", "residual", "weight", "bias")]
+        y = block(*t) if how == "plain" else checkpoint(block, *t, use_reentrant=reentrant)
+        y.backward(o["dy"])
+        results.append([y.detach()] + [v.grad for v in t])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@gpu
+def test_saved_tensors_elsewhere():
+    o = operands((50, 257), BF16, None, F32, "both", seed=24)
+    results = []
+    for hooks in (False, True):
+        x = o["x"].clone().requires_grad_()
+        if hooks:
+            with torch.autograd.graph.save_on_cpu():
+                y = layer_norm(x, o["weight"], o["bias"])
+        else:
+            y = layer_norm(x, o["weight"], o["bias"])
+        results.append(torch.autograd.grad(y, x, o["dy"])[0])
+    assert torch.equal(*results)
+
+
+@gpu
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwAD
+    x = torch.randn(4, 16, device="cuda")
+    with fwAD.dual_level():
+        d = fwAD.make_dual(x, torch.ones_like(x))
+        for call in (lambda: layer_norm(d), lambda: dropout(d, 0.5, 1), lambda: dropout_add_layer_norm(x, d)):
+            with pytest.raises(hip.HipError, match="forward-mode"):
+                call()
+
+
+@gpu
+def test_two_host_threads():
+    import threading
+    failed = []
+
+    def work(seed):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for k in range(8):
+                    check(operands((64 + seed, 130 + k), F32, F32, F32, "both", seed=seed * 100 + k), p=0.25, seed=k, offset=seed)
+        except BaseException as e:      # noqa: B902
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in (1, 2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not failed, failed
+
+
+@gpu
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_on_a_device_that_is_not_the_current_one():
+    o = operands((64, 256), F32, F32, F32, "both", seed=25)
+    there = {k: v.to("cuda:1") for k, v in o.items()}
+    torch.cuda.synchronize(0)
+    torch.cuda.synchronize(1)
+    check(there, p=0.25, seed=3)
+    with pytest.raises(hip.HipError):
+        dropout_add_layer_norm(there["x"], o["residual"])
+
+
+@gpu
 def test_block_of_the_tracker_trains():
     """A feed-forward block as the tracker has it -- norm(x + dropout(attn)), norm2(x + dropout(linear(dropout(gelu(linear(x)))))) -- with all
     gradients, against float64 autograd with the same masks.  The products run in float64 here, so what is off is the operators' own:
