@@ -145,6 +145,11 @@ __device__ __forceinline__ void keep_row(Keep8 (&m)[K], uint64_t e0, const DropK
   for (int k = 0; k < K; ++k) m[k] = keep_from(w[k], e0 + (uint32_t)((k * lanes + tl) * 8), key, tm1);
 }
 
+// May a half-precision row start in the middle of a dword?  Such rows of layer_norm are read dword by dword (Vec8, ODD): 24995 x 6001 f16
+// forward 126 -> 122 us, backward 241 -> 193; 36612 x 4097 143 -> 121 and 261 -> 221; 146914 x 1021 121 / 188 -> 121 / 180.  The join's are
+// not: its registers and instructions are what bounds it (148000 x 1021 187 / 328 us without, 212 / 332 with).
+inline bool odd_rows(const void* p, long long ld) { return (ld & 1) != 0 || (reinterpret_cast<uintptr_t>(p) & 2) != 0; }
+
 // calls f<TX, TR, RES>(a, s) for the types of a
 #define NORM_DISPATCH(F, a, s)                                                                            \
   do {                                                                                                    \

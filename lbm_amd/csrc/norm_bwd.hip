@@ -31,7 +31,7 @@ template <class TX, class TR, int K> struct BwdRow {
 // One row of a team: xhat and g = dy w from what was loaded, their two sums (s1 = sum g, s2 = sum g xhat), the columns' sums.
 // w: this thread's weights, from LDS where K > 1 (their registers would cost a wave a SIMD; a fetch is two ds_read_b128 a chunk).
 // gone: a row past the last one, of which nothing counts.
-template <class TX, class TR, int RES, int K, bool BLK>
+template <class TX, class TR, int RES, int K, bool BLK, bool ODD>
 __device__ __forceinline__ void bwd_row(const NormArgs& a, const DropKey& key, BwdRow<TX, TR, K>& in, const Span (&sp)[K], bool gone, long long row,
                                         int lanes, int tl, const float* w, float (&xh)[K][8], float (&g)[K][8], Keep8 (&m)[K],
                                         float (&dw)[K][8], float (&db)[K][8], float& s1, float& s2) {
@@ -39,9 +39,9 @@ __device__ __forceinline__ void bwd_row(const NormArgs& a, const DropKey& key, B
   if (RES && a.drop.on) keep_row<K, BLK>(m, (uint64_t)(row * a.cols), key, a.drop.tm1, (int)a.cols, lanes, tl);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    in.x[k].cut(sp[k].cut);
-    in.d[k].cut(gone ? 8 : sp[k].cut);
-    if (RES) in.r[k].cut(sp[k].cut);
+    in.x[k].template cut<ODD>(sp[k].cut);
+    in.d[k].template cut<ODD>(gone ? 8 : sp[k].cut);
+    if (RES) in.r[k].template cut<ODD>(sp[k].cut);
     if (RES && a.drop.on) {
       const uint32_t limit = keep_limit(a.drop.tm1);
 #pragma unroll
@@ -99,7 +99,7 @@ __device__ __forceinline__ void bwd_put(const NormArgs& a, const Span (&sp)[K], 
 }
 
 // Rows of lanes of a wave.  The next row's loads are issued when this row has become xhat and g, and pass behind its sums and stores.
-template <class TX, class TR, int RES, int K>
+template <class TX, class TR, int RES, int K, bool ODD>
 __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a, int shift) {
   __shared__ __align__(16) float red[4 * 512 * K];         // the weights (K > 1); at the end one column sum of every wave
   const int lanes = 1 << shift, tl = threadIdx.x & (lanes - 1), team = threadIdx.x >> shift, teams = 256 >> shift, cols = (int)a.cols;
@@ -128,9 +128,9 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a, int shift) {
     in.rstd = a.rstd[base + r];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      in.d[k].load(pd + row_at(r, (uint32_t)a.ld_dy, sp[k].at));
-      in.x[k].load(px + row_at(r, (uint32_t)a.ld_x, sp[k].at));
-      if (RES) in.r[k].load(pr + row_at(r, (uint32_t)a.ld_r, sp[k].at));
+      in.d[k].template load<ODD>(pd + row_at(r, (uint32_t)a.ld_dy, sp[k].at));
+      in.x[k].template load<ODD>(px + row_at(r, (uint32_t)a.ld_x, sp[k].at));
+      if (RES) in.r[k].template load<ODD>(pr + row_at(r, (uint32_t)a.ld_r, sp[k].at));
     }
   };
   const long long step = (long long)gridDim.x * teams;
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a, int shift) {
     float xh[K][8], g[K][8], s1, s2;
     Keep8 m[K];
     const float rstd = in.rstd;
-    bwd_row<TX, TR, RES, K, false>(a, key, in, sp, row >= a.rows, row, lanes, tl, K > 1 ? red : w, xh, g, m, dw, db, s1, s2);
+    bwd_row<TX, TR, RES, K, false, ODD>(a, key, in, sp, row >= a.rows, row, lanes, tl, K > 1 ? red : w, xh, g, m, dw, db, s1, s2);
     if (base + step < a.rows) load(base + step);
     const float c1 = lanes_sum(s1, shift) * inv, c2 = lanes_sum(s2, shift) * inv;
     if (row < a.rows) bwd_put<TX, TR, RES, K>(a, sp, row * a.cols, lanes, tl, c1, c2, rstd, xh, g, m);
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a, int shift) {
 
 // Rows of a workgroup.  AHEAD: the next row's loads pass behind this row's sums, as above, at the price of registers (512 threads at
 // most); otherwise up to 1024 threads with 128 registers each, a row at a time.
-template <class TX, class TR, int RES, int K, bool AHEAD>
+template <class TX, class TR, int RES, int K, bool AHEAD, bool ODD>
 __global__ __launch_bounds__(AHEAD ? 512 : 1024) void norm_bwd_block_kernel(NormArgs a) {
   extern __shared__ __align__(16) float wlds[];            // K * blockDim.x * 8 weights
   __shared__ float sums[2][16][2];
@@ -198,9 +198,9 @@ __global__ __launch_bounds__(AHEAD ? 512 : 1024) void norm_bwd_block_kernel(Norm
     in.rstd = a.rstd[row];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      in.d[k].load(pd + sp[k].at);
-      in.x[k].load(px + sp[k].at);
-      if (RES) in.r[k].load(pr + sp[k].at);
+      in.d[k].template load<ODD>(pd + sp[k].at);
+      in.x[k].template load<ODD>(px + sp[k].at);
+      if (RES) in.r[k].template load<ODD>(pr + sp[k].at);
     }
   };
   if (AHEAD && blockIdx.x < a.rows) load(blockIdx.x);
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(AHEAD ? 512 : 1024) void norm_bwd_block_kernel(Norm
     float xh[K][8], g[K][8], s1, s2;
     Keep8 m[K];
     const float rstd = in.rstd;
-    bwd_row<TX, TR, RES, K, true>(a, key, in, sp, false, row, lanes, tl, wlds, xh, g, m, dw, db, s1, s2);
+    bwd_row<TX, TR, RES, K, true, ODD>(a, key, in, sp, false, row, lanes, tl, wlds, xh, g, m, dw, db, s1, s2);
     if (AHEAD && row + gridDim.x < a.rows) load(row + gridDim.x);
     // one barrier a row: the next row writes the other half, and the one after it finds every thread past this row's reads
     s1 = wave64_sum(s1);
@@ -296,21 +296,27 @@ uint64_t norm_workspace_bytes(long long rows, long long cols) {
   return (uint64_t)parts * 2 * (uint64_t)cols * sizeof(float);
 }
 
-template <class TX, class TR, int RES> static int backward(const NormArgs& a, hipStream_t s) {
+template <class TX, class TR, int RES, bool ODD> static int backward_rows(const NormArgs& a, hipStream_t s) {
   constexpr bool lean = RES == 0 && sizeof(TX) == 2;
   const NormShape sh = bwd_shape(a.cols, lean);
   const int grid = norm_parts(a.rows, a.cols, lean);
   const size_t lds = (size_t)sh.threads * sh.k * 8 * sizeof(float);
-  if (sh.block && sh.k == 4) norm_bwd_block_kernel<TX, TR, RES, lean ? 4 : 2, true><<<grid, sh.threads, lds, s>>>(a);
-  else if (sh.block && sh.threads <= 512) norm_bwd_block_kernel<TX, TR, RES, 2, true><<<grid, sh.threads, lds, s>>>(a);
-  else if (sh.block) norm_bwd_block_kernel<TX, TR, RES, 2, false><<<grid, sh.threads, lds, s>>>(a);
-  else if (sh.k == 1) norm_bwd_kernel<TX, TR, RES, 1><<<grid, 256, 0, s>>>(a, sh.shift);
-  else if (sh.k == 2) norm_bwd_kernel<TX, TR, RES, 2><<<grid, 256, 0, s>>>(a, sh.shift);
-  else if (sh.k == 3) norm_bwd_kernel<TX, TR, RES, 3><<<grid, 256, 0, s>>>(a, sh.shift);
-  else norm_bwd_kernel<TX, TR, RES, 4><<<grid, 256, 0, s>>>(a, sh.shift);
+  if (sh.block && sh.k == 4) norm_bwd_block_kernel<TX, TR, RES, lean ? 4 : 2, true, ODD><<<grid, sh.threads, lds, s>>>(a);
+  else if (sh.block && sh.threads <= 512) norm_bwd_block_kernel<TX, TR, RES, 2, true, ODD><<<grid, sh.threads, lds, s>>>(a);
+  else if (sh.block) norm_bwd_block_kernel<TX, TR, RES, 2, false, ODD><<<grid, sh.threads, lds, s>>>(a);
+  else if (sh.k == 1) norm_bwd_kernel<TX, TR, RES, 1, ODD><<<grid, 256, 0, s>>>(a, sh.shift);
+  else if (sh.k == 2) norm_bwd_kernel<TX, TR, RES, 2, ODD><<<grid, 256, 0, s>>>(a, sh.shift);
+  else if (sh.k == 3) norm_bwd_kernel<TX, TR, RES, 3, ODD><<<grid, 256, 0, s>>>(a, sh.shift);
+  else norm_bwd_kernel<TX, TR, RES, 4, ODD><<<grid, 256, 0, s>>>(a, sh.shift);
   if (check_launch("norm_backward")) return -1;
   if (grid > 1 && (a.dweight != nullptr || a.dbias != nullptr)) return norm_finish(a, grid, s);
   return 0;
+}
+
+template <class TX, class TR, int RES> static int backward(const NormArgs& a, hipStream_t s) {
+  constexpr bool can = RES == 0 && sizeof(TX) == 2;      // (norm.hpp, odd_rows)
+  if (can && (odd_rows(a.x, a.ld_x) || odd_rows(a.dy, a.ld_dy))) return backward_rows<TX, TR, RES, can>(a, s);
+  return backward_rows<TX, TR, RES, false>(a, s);
 }
 
 int norm_backward(const NormArgs& a, hipStream_t stream) {

@@ -11,7 +11,7 @@ template <class TX, class TR, int K> struct FwdRow {
 };
 
 // z of a loaded row, its sum in s
-template <class TX, class TR, int RES, int K, bool BLK>
+template <class TX, class TR, int RES, int K, bool BLK, bool ODD>
 __device__ __forceinline__ float join_row(const NormArgs& a, const DropKey& key, FwdRow<TX, TR, K>& in, const Span (&sp)[K], long long row,
                                           int lanes, int tl, float (&z)[K][8]) {
   float s = 0.0f;
@@ -19,8 +19,8 @@ __device__ __forceinline__ float join_row(const NormArgs& a, const DropKey& key,
   if (RES && a.drop.on) keep_row<K, BLK>(m, (uint64_t)(row * a.cols), key, a.drop.tm1, (int)a.cols, lanes, tl);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    in.x[k].cut(sp[k].cut);
-    if (RES) in.r[k].cut(sp[k].cut);
+    in.x[k].template cut<ODD>(sp[k].cut);
+    if (RES) in.r[k].template cut<ODD>(sp[k].cut);
     if (RES && a.drop.on) {
       const uint32_t limit = keep_limit(a.drop.tm1);
 #pragma unroll
@@ -60,7 +60,7 @@ template <class TR> __device__ __forceinline__ void put_y(TR* y, float (&z)[8], 
 
 // Rows of up to 2048 columns.  U rows a team are loaded before the first is used, and a workgroup ends after them: a grid in row order
 // keeps the whole chip on neighbouring pages.
-template <class TX, class TR, int RES, int K, int U>
+template <class TX, class TR, int RES, int K, int U, bool ODD>
 __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift) {
   const int lanes = 1 << shift, tl = threadIdx.x & (lanes - 1), team = threadIdx.x >> shift, teams = 256 >> shift, cols = (int)a.cols;
   const float inv = 1.0f / (float)cols;
@@ -80,8 +80,8 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift) {
     const uint32_t r = min(u * teams + team, last);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      in[u].x[k].load(px + row_at(r, (uint32_t)a.ld_x, sp[k].at));
-      if (RES) in[u].r[k].load(pr + row_at(r, (uint32_t)a.ld_r, sp[k].at));
+      in[u].x[k].template load<ODD>(px + row_at(r, (uint32_t)a.ld_x, sp[k].at));
+      if (RES) in[u].r[k].template load<ODD>(pr + row_at(r, (uint32_t)a.ld_r, sp[k].at));
     }
   }
   float w[K][8], b[K][8];
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift) {
   for (int u = 0; u < U; ++u) {
     const int r = u * teams + team;
     float z[K][8];
-    const float mean = lanes_sum(join_row<TX, TR, RES, K, false>(a, key, in[u], sp, base + r, lanes, tl, z), shift) * inv;
+    const float mean = lanes_sum(join_row<TX, TR, RES, K, false, ODD>(a, key, in[u], sp, base + r, lanes, tl, z), shift) * inv;
     const float rstd = rsqrt_newton(lanes_sum(deviate<K>(z, mean, sp), shift) * inv + a.eps);
     if (r > last) continue;
     if (tl == 0 && a.mean != nullptr) {
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift) {
 
 // Rows of a workgroup.  The next row's loads are issued when this row has become z, so they pass behind its two sums and its stores: with
 // 512 or 1024 threads a row only one or two rows are on a CU, and without that its memory was idle half of the time.
-template <class TX, class TR, int RES, int K>
+template <class TX, class TR, int RES, int K, bool ODD>
 __global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
   __shared__ float sm[2][16];
   const int lanes = blockDim.x, tl = threadIdx.x, cols = (int)a.cols;
@@ -125,8 +125,8 @@ __global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
     const TR* pr = reinterpret_cast<const TR*>(a.residual) + row * a.ld_r;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      in.x[k].load(px + sp[k].at);
-      if (RES) in.r[k].load(pr + sp[k].at);
+      in.x[k].template load<ODD>(px + sp[k].at);
+      if (RES) in.r[k].template load<ODD>(pr + sp[k].at);
     }
   };
   float w[K][8], b[K][8];
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
   }
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     float z[K][8];
-    const float s = join_row<TX, TR, RES, K, true>(a, key, in, sp, row, lanes, tl, z);
+    const float s = join_row<TX, TR, RES, K, true, ODD>(a, key, in, sp, row, lanes, tl, z);
     if (row + gridDim.x < a.rows) load(row + gridDim.x);
     const float mean = block_sum(s, sm[0]) * inv;
     const float rstd = rsqrt_newton(block_sum(deviate<K>(z, mean, sp), sm[1]) * inv + a.eps);
@@ -157,25 +157,30 @@ __global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
 #define NF_MANY 2048
 #define NF_JOIN 128
 #endif
-template <class TX, class TR, int RES, int K, int U> static int wave_forward(const NormArgs& a, const NormShape& sh, hipStream_t s) {
+template <class TX, class TR, int RES, int K, int U, bool ODD> static int wave_forward(const NormArgs& a, const NormShape& sh, hipStream_t s) {
   const long long per = (long long)sh.teams() * U, grid = (a.rows + per - 1) / per;
   LBM_REQUIRE(grid < (1ll << 31), "norm_forward: %lld rows are more than a grid holds", a.rows);
-  norm_fwd_kernel<TX, TR, RES, K, U><<<(unsigned)grid, 256, 0, s>>>(a, sh.shift);
+  norm_fwd_kernel<TX, TR, RES, K, U, ODD><<<(unsigned)grid, 256, 0, s>>>(a, sh.shift);
   return check_launch("norm_forward");
 }
-template <class TX, class TR, int RES> static int forward(const NormArgs& a, hipStream_t s) {
+template <class TX, class TR, int RES, bool ODD> static int forward_rows(const NormArgs& a, hipStream_t s) {
   const NormShape sh = norm_shape(a.cols, RES ? NF_JOIN : 256);
   if (sh.block) {
     const long long most = 256 * (1024 / sh.threads);      // what is resident at once (16 waves a CU), a whole number a CU
-    norm_fwd_block_kernel<TX, TR, RES, 2><<<(unsigned)(a.rows < most ? a.rows : most), sh.threads, 0, s>>>(a);
+    norm_fwd_block_kernel<TX, TR, RES, 2, ODD><<<(unsigned)(a.rows < most ? a.rows : most), sh.threads, 0, s>>>(a);
     return check_launch("norm_forward");
   }
   constexpr int U1 = RES ? 2 : 4, U2 = RES ? 1 : 2;
-  if (sh.k == 4) return wave_forward<TX, TR, RES, 4, 1>(a, sh, s);
+  if (sh.k == 4) return wave_forward<TX, TR, RES, 4, 1, ODD>(a, sh, s);
   const bool many = a.rows >= (long long)sh.teams() * (sh.k == 1 ? U1 : U2) * NF_MANY;
-  if (sh.k == 1) return many ? wave_forward<TX, TR, RES, 1, U1>(a, sh, s) : wave_forward<TX, TR, RES, 1, 1>(a, sh, s);
-  if (sh.k == 2) return many ? wave_forward<TX, TR, RES, 2, U2>(a, sh, s) : wave_forward<TX, TR, RES, 2, 1>(a, sh, s);
-  return many ? wave_forward<TX, TR, RES, 3, U2>(a, sh, s) : wave_forward<TX, TR, RES, 3, 1>(a, sh, s);
+  if (sh.k == 1) return many ? wave_forward<TX, TR, RES, 1, U1, ODD>(a, sh, s) : wave_forward<TX, TR, RES, 1, 1, ODD>(a, sh, s);
+  if (sh.k == 2) return many ? wave_forward<TX, TR, RES, 2, U2, ODD>(a, sh, s) : wave_forward<TX, TR, RES, 2, 1, ODD>(a, sh, s);
+  return many ? wave_forward<TX, TR, RES, 3, U2, ODD>(a, sh, s) : wave_forward<TX, TR, RES, 3, 1, ODD>(a, sh, s);
+}
+template <class TX, class TR, int RES> static int forward(const NormArgs& a, hipStream_t s) {
+  constexpr bool can = RES == 0 && sizeof(TX) == 2;      // (norm.hpp, odd_rows)
+  if (can && odd_rows(a.x, a.ld_x)) return forward_rows<TX, TR, RES, can>(a, s);
+  return forward_rows<TX, TR, RES, false>(a, s);
 }
 
 int norm_forward(const NormArgs& a, hipStream_t stream) {
