@@ -10,15 +10,25 @@
 
 namespace lbm {
 
-// dweight / dbias from the first partial sum when it is the only one
-template <class T> __device__ __forceinline__ void put_sum(const NormArgs& a, int which, long long c, float v) {
-  T* o = reinterpret_cast<T*>(which == 0 ? a.dweight : a.dbias);
-  if (o != nullptr) o[c] = (T)v;
+// Where a workgroup's column sums go: its partial sum, or dweight / dbias themselves when there is only one workgroup.
+template <class T> __device__ __forceinline__ void put_sum(void* p, long long c, float v) {
+  if (p != nullptr) reinterpret_cast<T*>(p)[c] = (T)v;
 }
 template <class TX> __device__ __forceinline__ void put_part(const NormArgs& a, int which, long long c, float v) {
   if (gridDim.x > 1) a.workspace[((long long)blockIdx.x * 2 + which) * a.cols + c] = v;
-  else if (a.p_f32) put_sum<float>(a, which, c, v);
-  else put_sum<TX>(a, which, c, v);
+  else if (a.p_f32) put_sum<float>(which == 0 ? a.dweight : a.dbias, c, v);
+  else put_sum<TX>(which == 0 ? a.dweight : a.dbias, c, v);
+}
+template <class T> __device__ __forceinline__ void put_sums(void* p, long long c, const float (&v)[8], int nv) {
+  if (p == nullptr) return;
+  Vec8<T> o;
+  o.set(v);
+  o.store(reinterpret_cast<T*>(p) + c, nv);
+}
+template <class TX> __device__ __forceinline__ void put_parts(const NormArgs& a, int which, long long c, const float (&v)[8], int nv) {
+  if (gridDim.x > 1) put_sums<float>(a.workspace + ((long long)blockIdx.x * 2 + which) * a.cols, c, v, nv);
+  else if (a.p_f32) put_sums<float>(which == 0 ? a.dweight : a.dbias, c, v, nv);
+  else put_sums<TX>(which == 0 ? a.dweight : a.dbias, c, v, nv);
 }
 
 template <class TX, class TR, int K> struct BwdRow {
@@ -231,12 +241,10 @@ __global__ __launch_bounds__(AHEAD ? 512 : 1024) void norm_bwd_block_kernel(Norm
   if (a.dweight == nullptr && a.dbias == nullptr) return;
 #pragma unroll
   for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < 8 - sp[k].cut) {
-        put_part<TX>(a, 0, (k * lanes + tl) * 8 + j, dw[k][j]);
-        put_part<TX>(a, 1, (k * lanes + tl) * 8 + j, db[k][j]);
-      }
+    if (sp[k].cut < 8) {
+      put_parts<TX>(a, 0, (k * lanes + tl) * 8, dw[k], 8 - sp[k].cut);
+      put_parts<TX>(a, 1, (k * lanes + tl) * 8, db[k], 8 - sp[k].cut);
+    }
 }
 
 // dweight / dbias = the partial sums added up in a fixed order: 32 columns x 32 slices of the partial sums a workgroup
@@ -270,12 +278,13 @@ int norm_finish(const NormArgs& a, int parts, hipStream_t s) {
   return check_launch("norm_backward");
 }
 
-// The teams of the backward pass: more than 1024 columns belong to a workgroup (K = 4 in a wave leaves one wave a SIMD).  Up to 8192 columns
+// The teams of the backward pass: more than 1536 columns belong to a workgroup (K = 4 in a wave leaves one wave a SIMD; between 1024 and
+// 1536 a wave's 192 chunks waste less than a workgroup's 256: the join at 145348 x 1032 bf16 314 us, 504 in a workgroup).  Up to 8192 columns
 // it has 512 threads at most, with registers for the loads ahead; beyond, K = 4 chunks a thread where they fit beside those (lean: half
 // precision without a residual), else 1024 threads that load a row at a time.
 static NormShape bwd_shape(long long cols, bool lean) {
   const int chunks = (int)((cols + 7) / 8);
-  if (chunks <= 128) return norm_shape(cols, 128);
+  if (chunks <= 192) return norm_shape(cols, 192);
   NormShape s{chunks > 1024 && lean ? 4 : 2, 0, 0, true};
   s.threads = (chunks + 64 * s.k - 1) / (64 * s.k) * 64;
   return s;
@@ -287,7 +296,7 @@ static int norm_parts(long long rows, long long cols, bool lean) {
   if (sh.block) per_cu = sh.threads <= 128 ? 3 : sh.threads <= 256 ? 2 : 1;
   while (sh.block && per_cu > 1 && rows < 8 * 256 * per_cu) --per_cu;      // a partial sum costs as much traffic as four rows
   const long long g = (rows + sh.teams() - 1) / sh.teams();
-  if (g <= 8) return 1;                    // a few rounds of one workgroup cost less than the second launch
+  if (g <= (sh.block || sh.k > 1 ? 2 : 8)) return 1;       // a few rounds of one workgroup (64 x 256: 7.5 us) cost no more than the second launch (6.3 - 9)
   return (int)std::min(g, 256ll * per_cu);
 }
 

@@ -153,10 +153,12 @@ __global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
   }
 }
 
-#ifndef NF_MANY
-#define NF_MANY 2048
-#define NF_JOIN 128
-#endif
+// Rows in flight a team: four (the join two) when that still makes 2048 workgroups, else one (65536 x 256 f16: 14.3 us with four, 15.8 with
+// one; the join at 9216 x 256: 9.0 us with four, 6.9 with one).
+constexpr long long kManyGroups = 2048;
+// Chunks that a wave may hold: the join's four a lane leave two waves a SIMD (93750 x 1600 bf16: 218 us, 181 in a workgroup), three do not
+// (97656 x 1536: 156 us, 179 in a workgroup).
+template <int RES> constexpr int wave_chunks() { return RES ? 192 : 256; }
 template <class TX, class TR, int RES, int K, int U, bool ODD> static int wave_forward(const NormArgs& a, const NormShape& sh, hipStream_t s) {
   const long long per = (long long)sh.teams() * U, grid = (a.rows + per - 1) / per;
   LBM_REQUIRE(grid < (1ll << 31), "norm_forward: %lld rows are more than a grid holds", a.rows);
@@ -164,7 +166,7 @@ template <class TX, class TR, int RES, int K, int U, bool ODD> static int wave_f
   return check_launch("norm_forward");
 }
 template <class TX, class TR, int RES, bool ODD> static int forward_rows(const NormArgs& a, hipStream_t s) {
-  const NormShape sh = norm_shape(a.cols, RES ? NF_JOIN : 256);
+  const NormShape sh = norm_shape(a.cols, wave_chunks<RES>());
   if (sh.block) {
     const long long most = 256 * (1024 / sh.threads);      // what is resident at once (16 waves a CU), a whole number a CU
     norm_fwd_block_kernel<TX, TR, RES, 2, ODD><<<(unsigned)(a.rows < most ? a.rows : most), sh.threads, 0, s>>>(a);
@@ -172,7 +174,7 @@ template <class TX, class TR, int RES, bool ODD> static int forward_rows(const N
   }
   constexpr int U1 = RES ? 2 : 4, U2 = RES ? 1 : 2;
   if (sh.k == 4) return wave_forward<TX, TR, RES, 4, 1, ODD>(a, sh, s);
-  const bool many = a.rows >= (long long)sh.teams() * (sh.k == 1 ? U1 : U2) * NF_MANY;
+  const bool many = a.rows >= (long long)sh.teams() * (sh.k == 1 ? U1 : U2) * kManyGroups;
   if (sh.k == 1) return many ? wave_forward<TX, TR, RES, 1, U1, ODD>(a, sh, s) : wave_forward<TX, TR, RES, 1, 1, ODD>(a, sh, s);
   if (sh.k == 2) return many ? wave_forward<TX, TR, RES, 2, U2, ODD>(a, sh, s) : wave_forward<TX, TR, RES, 2, 1, ODD>(a, sh, s);
   return many ? wave_forward<TX, TR, RES, 3, U2, ODD>(a, sh, s) : wave_forward<TX, TR, RES, 3, 1, ODD>(a, sh, s);
