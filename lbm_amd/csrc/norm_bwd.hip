@@ -296,7 +296,7 @@ static int norm_parts(long long rows, long long cols, bool lean) {
   if (sh.block) per_cu = sh.threads <= 128 ? 3 : sh.threads <= 256 ? 2 : 1;
   while (sh.block && per_cu > 1 && rows < 8 * 256 * per_cu) --per_cu;      // a partial sum costs as much traffic as four rows
   const long long g = (rows + sh.teams() - 1) / sh.teams();
-  if (g <= (sh.block || sh.k > 1 ? 2 : 8)) return 1;       // a few rounds of one workgroup (64 x 256: 7.5 us) cost no more than the second launch (6.3 - 9)
+  if (g <= (sh.block || sh.k > 1 ? 2 : 4)) return 1;       // a few rounds of one workgroup (32 x 256: 5.3 us) cost less than the second launch (8.4)
   return (int)std::min(g, 256ll * per_cu);
 }
 

@@ -375,6 +375,7 @@ PYBIND11_MODULE(_torch_ops, m) {
   // differentiable
   m.def("dropout", [](const Tensor& x, double p, uint64_t seed, const Maybe& seed_dev, uint64_t offset) -> Tensor {
     HANDLE_TH_ERRORS
+    const py::gil_scoped_release no_gil;         // allocations and launches may wait
     elem_type(x, "dropout");
     return dropout(x, make_drop("dropout", p, seed, seed_dev, offset, x));
     END_HANDLE_TH_ERRORS_PYBIND
@@ -382,6 +383,7 @@ PYBIND11_MODULE(_torch_ops, m) {
   m.def("norm", [](const Tensor& x, const Maybe& residual, const Maybe& weight, const Maybe& bias, double eps, double p, uint64_t seed,
                    const Maybe& seed_dev, uint64_t offset) -> Tensor {
     HANDLE_TH_ERRORS
+    const py::gil_scoped_release no_gil;         // allocations and launches may wait
     const char* what = residual.has_value() ? "dropout_add_layer_norm" : "layer_norm";
     return norm(what, x, get(residual), get(weight), get(bias), eps, make_drop(what, p, seed, seed_dev, offset, x));
     END_HANDLE_TH_ERRORS_PYBIND
@@ -389,6 +391,7 @@ PYBIND11_MODULE(_torch_ops, m) {
   // single passes
   m.def("dropout_pass", [](const Tensor& x, double p, uint64_t seed, const Maybe& seed_dev, uint64_t offset) -> Tensor {
     HANDLE_TH_ERRORS
+    const py::gil_scoped_release no_gil;         // allocations and launches may wait
     const c10::AutoGradMode off(false);
     elem_type(x, "dropout");
     return run_dropout(x, make_drop("dropout", p, seed, seed_dev, offset, x));
@@ -397,6 +400,7 @@ PYBIND11_MODULE(_torch_ops, m) {
   m.def("norm_forward", [](const Tensor& x, const Maybe& residual, const Maybe& weight, const Maybe& bias, double eps, double p, uint64_t seed,
                            const Maybe& seed_dev, uint64_t offset, bool want_stats) -> std::tuple<Tensor, Tensor> {
     HANDLE_TH_ERRORS
+    const py::gil_scoped_release no_gil;         // allocations and launches may wait
     const c10::AutoGradMode off(false);
     const Operands o = operands("norm_forward", x, get(residual), get(weight), get(bias));
     return run_forward(o, eps, make_drop("norm_forward", p, seed, seed_dev, offset, x), want_stats);
@@ -406,6 +410,7 @@ PYBIND11_MODULE(_torch_ops, m) {
                             const Maybe& bias, double eps, double p, uint64_t seed, const Maybe& seed_dev, uint64_t offset, bool want_x,
                             bool want_r, bool want_w, bool want_b) -> variable_list {
     HANDLE_TH_ERRORS
+    const py::gil_scoped_release no_gil;         // allocations and launches may wait
     const c10::AutoGradMode off(false);
     const Operands o = operands("norm_backward", x, get(residual), get(weight), get(bias));
     const Tensor& like = residual.has_value() ? *residual : x;
