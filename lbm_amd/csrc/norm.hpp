@@ -4,8 +4,7 @@
 
 namespace lbm {
 
-// rows that a team holds in registers; shorter (no eight elements to read at once) and longer ones: norm_wide.hip
-constexpr long long kNormRowMin = 8, kNormRowMax = 16384;
+constexpr long long kNormRowMax = 16384;      // longest row that a team holds in registers; beyond: norm_wide.hip
 
 int norm_wide_forward(const NormArgs& a, hipStream_t stream);
 int norm_wide_backward(const NormArgs& a, hipStream_t stream);
@@ -45,26 +44,34 @@ inline NormShape norm_shape(long long cols, int most) {        // most: chunks t
 }
 
 // Where a chunk's eight elements are read: the last one of a row that is no multiple of eight is read from eight before the row's end on
-// and cut, so no load lies outside of the row and none waits for a branch.  cut = 8: the chunk lies past the row's end.
+// and cut, so no load lies outside of the row and none waits for a branch.  cut = 8: the chunk lies past the row's end.  (Rows of fewer
+// than eight elements are a chunk that is loaded element by element, with cut = 8 - cols.)  Only a thread's last chunk can be cut: a team
+// has no more chunks than it needs, (K - 1) T < ceil(cols / 8) for every shape above, so chunk k < K - 1 is whole and costs no test.
 struct Span {
   int at, cut;
   __device__ __forceinline__ Span() {}
-  __device__ __forceinline__ Span(int c, int cols) : at(min(c, cols - 8)), cut(min(c - at, 8)) {}
+  __device__ __forceinline__ Span(int a, int c) : at(a), cut(c) {}
+  template <LoadMode MODE> static __device__ __forceinline__ Span of(int c, int cols, bool last) {
+    if (!last) return Span(c, 0);
+    if (MODE == kShort) return Span(0, c == 0 ? 8 - cols : 8);
+    const int at = min(c, cols - 8);
+    return Span(at, min(c - at, 8));
+  }
 };
-template <class TX> __device__ __forceinline__ void load_param(const void* p, int p_f32, const Span& s, float dflt, float (&v)[8]) {
+template <class TX, LoadMode MODE> __device__ __forceinline__ void load_param(const void* p, int p_f32, const Span& s, float dflt, float (&v)[8]) {
   if (p == nullptr) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = dflt;
   } else if (p_f32) {
     Vec8<float> r;
-    r.load(reinterpret_cast<const float*>(p) + s.at);
-    r.cut(s.cut);
+    r.template load<MODE>(reinterpret_cast<const float*>(p) + s.at, 8 - s.cut);
+    r.template cut<MODE>(s.cut);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = r.get(j);
   } else {
     Vec8<TX> r;
-    r.load(reinterpret_cast<const TX*>(p) + s.at);
-    r.cut(s.cut);
+    r.template load<MODE>(reinterpret_cast<const TX*>(p) + s.at, 8 - s.cut);
+    r.template cut<MODE>(s.cut);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = r.get(j);
   }
@@ -145,10 +152,9 @@ __device__ __forceinline__ void keep_row(Keep8 (&m)[K], uint64_t e0, const DropK
   for (int k = 0; k < K; ++k) m[k] = keep_from(w[k], e0 + (uint32_t)((k * lanes + tl) * 8), key, tm1);
 }
 
-// May a half-precision row start in the middle of a dword?  Such rows of layer_norm are read dword by dword (Vec8, ODD): 24995 x 6001 f16
-// forward 126 -> 122 us, backward 241 -> 193; 36612 x 4097 143 -> 121 and 261 -> 221; 146914 x 1021 121 / 188 -> 121 / 180.  The join's are
-// not: its registers and instructions are what bounds it (148000 x 1021 187 / 328 us without, 212 / 332 with).
-inline bool odd_rows(const void* p, long long ld) { return (ld & 1) != 0 || (reinterpret_cast<uintptr_t>(p) & 2) != 0; }
+// May a half-precision row start in the middle of a dword?  Such rows are read dword by dword (Vec8, kOdd): 24995 x 6001 f16 forward 126 -> 122 us,
+// backward 241 -> 193; 36612 x 4097 143 -> 121 and 261 -> 221; the join at 18312 x 8191 bf16 195 -> 170 and 367 -> 285, 73277 x 2047 208 -> 183 and 387 -> 309.
+template <class T> inline bool odd_rows(const void* p, long long ld) { return sizeof(T) == 2 && ((ld & 1) != 0 || (reinterpret_cast<uintptr_t>(p) & 2) != 0); }
 
 // calls f<TX, TR, RES>(a, s) for the types of a
 #define NORM_DISPATCH(F, a, s)                                                                            \

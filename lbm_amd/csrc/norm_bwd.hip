@@ -41,7 +41,7 @@ template <class TX, class TR, int K> struct BwdRow {
 // One row of a team: xhat and g = dy w from what was loaded, their two sums (s1 = sum g, s2 = sum g xhat), the columns' sums.
 // w: this thread's weights, from LDS where K > 1 (their registers would cost a wave a SIMD; a fetch is two ds_read_b128 a chunk).
 // gone: a row past the last one, of which nothing counts.
-template <class TX, class TR, int RES, int K, bool BLK, bool ODD>
+template <class TX, class TR, int RES, int K, bool BLK, LoadMode MODE>
 __device__ __forceinline__ void bwd_row(const NormArgs& a, const DropKey& key, BwdRow<TX, TR, K>& in, const Span (&sp)[K], bool gone, long long row,
                                         int lanes, int tl, const float* w, float (&xh)[K][8], float (&g)[K][8], Keep8 (&m)[K],
                                         float (&dw)[K][8], float (&db)[K][8], float& s1, float& s2) {
@@ -49,9 +49,9 @@ __device__ __forceinline__ void bwd_row(const NormArgs& a, const DropKey& key, B
   if (RES && a.drop.on) keep_row<K, BLK>(m, (uint64_t)(row * a.cols), key, a.drop.tm1, (int)a.cols, lanes, tl);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    in.x[k].template cut<ODD>(sp[k].cut);
-    in.d[k].template cut<ODD>(gone ? 8 : sp[k].cut);
-    if (RES) in.r[k].template cut<ODD>(sp[k].cut);
+    in.x[k].template cut<MODE>(sp[k].cut);
+    in.d[k].template cut<MODE>(gone ? 8 : sp[k].cut);
+    if (RES) in.r[k].template cut<MODE>(sp[k].cut);
     if (RES && a.drop.on) {
       const uint32_t limit = keep_limit(a.drop.tm1);
 #pragma unroll
@@ -109,7 +109,7 @@ __device__ __forceinline__ void bwd_put(const NormArgs& a, const Span (&sp)[K], 
 }
 
 // Rows of lanes of a wave.  The next row's loads are issued when this row has become xhat and g, and pass behind its sums and stores.
-template <class TX, class TR, int RES, int K, bool ODD>
+template <class TX, class TR, int RES, int K, LoadMode MODE>
 __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a, int shift) {
   __shared__ __align__(16) float red[4 * 512 * K];         // the weights (K > 1); at the end one column sum of every wave
   const int lanes = 1 << shift, tl = threadIdx.x & (lanes - 1), team = threadIdx.x >> shift, teams = 256 >> shift, cols = (int)a.cols;
@@ -120,8 +120,8 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a, int shift) {
   float w[8], dw[K][8] = {}, db[K][8] = {};
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    sp[k] = Span((k * lanes + tl) * 8, cols);
-    if (K == 1 || (int)threadIdx.x < lanes) load_param<TX>(a.weight, a.p_f32, sp[k], 1.0f, w);
+    sp[k] = Span::of<MODE>((k * lanes + tl) * 8, cols, k == K - 1);
+    if (K == 1 || (int)threadIdx.x < lanes) load_param<TX, MODE == kShort ? kShort : kPlain>(a.weight, a.p_f32, sp[k], 1.0f, w);
     if (K > 1 && (int)threadIdx.x < lanes) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) red[(k * lanes + tl) * 8 + j] = w[j];
@@ -138,9 +138,9 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a, int shift) {
     in.rstd = a.rstd[base + r];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      in.d[k].template load<ODD>(pd + row_at(r, (uint32_t)a.ld_dy, sp[k].at));
-      in.x[k].template load<ODD>(px + row_at(r, (uint32_t)a.ld_x, sp[k].at));
-      if (RES) in.r[k].template load<ODD>(pr + row_at(r, (uint32_t)a.ld_r, sp[k].at));
+      in.d[k].template load<MODE>(pd + row_at(r, (uint32_t)a.ld_dy, sp[k].at), 8 - sp[k].cut);
+      in.x[k].template load<MODE>(px + row_at(r, (uint32_t)a.ld_x, sp[k].at), 8 - sp[k].cut);
+      if (RES) in.r[k].template load<MODE>(pr + row_at(r, (uint32_t)a.ld_r, sp[k].at), 8 - sp[k].cut);
     }
   };
   const long long step = (long long)gridDim.x * teams;
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a, int shift) {
     float xh[K][8], g[K][8], s1, s2;
     Keep8 m[K];
     const float rstd = in.rstd;
-    bwd_row<TX, TR, RES, K, false, ODD>(a, key, in, sp, row >= a.rows, row, lanes, tl, K > 1 ? red : w, xh, g, m, dw, db, s1, s2);
+    bwd_row<TX, TR, RES, K, false, MODE>(a, key, in, sp, row >= a.rows, row, lanes, tl, K > 1 ? red : w, xh, g, m, dw, db, s1, s2);
     if (base + step < a.rows) load(base + step);
     const float c1 = lanes_sum(s1, shift) * inv, c2 = lanes_sum(s2, shift) * inv;
     if (row < a.rows) bwd_put<TX, TR, RES, K>(a, sp, row * a.cols, lanes, tl, c1, c2, rstd, xh, g, m);
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a, int shift) {
 
 // Rows of a workgroup.  AHEAD: the next row's loads pass behind this row's sums, as above, at the price of registers (512 threads at
 // most); otherwise up to 1024 threads with 128 registers each, a row at a time.
-template <class TX, class TR, int RES, int K, bool AHEAD, bool ODD>
+template <class TX, class TR, int RES, int K, bool AHEAD, LoadMode MODE>
 __global__ __launch_bounds__(AHEAD ? 512 : 1024) void norm_bwd_block_kernel(NormArgs a) {
   extern __shared__ __align__(16) float wlds[];            // K * blockDim.x * 8 weights
   __shared__ float sums[2][16][2];
@@ -194,8 +194,8 @@ __global__ __launch_bounds__(AHEAD ? 512 : 1024) void norm_bwd_block_kernel(Norm
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     float w[8];
-    sp[k] = Span((k * lanes + tl) * 8, cols);
-    load_param<TX>(a.weight, a.p_f32, sp[k], 1.0f, w);
+    sp[k] = Span::of<MODE>((k * lanes + tl) * 8, cols, k == K - 1);
+    load_param<TX, MODE == kShort ? kShort : kPlain>(a.weight, a.p_f32, sp[k], 1.0f, w);
 #pragma unroll
     for (int j = 0; j < 8; ++j) wlds[(k * lanes + tl) * 8 + j] = w[j];      // read by this thread only
   }
@@ -208,9 +208,9 @@ __global__ __launch_bounds__(AHEAD ? 512 : 1024) void norm_bwd_block_kernel(Norm
     in.rstd = a.rstd[row];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      in.d[k].template load<ODD>(pd + sp[k].at);
-      in.x[k].template load<ODD>(px + sp[k].at);
-      if (RES) in.r[k].template load<ODD>(pr + sp[k].at);
+      in.d[k].template load<MODE>(pd + sp[k].at, 8 - sp[k].cut);
+      in.x[k].template load<MODE>(px + sp[k].at, 8 - sp[k].cut);
+      if (RES) in.r[k].template load<MODE>(pr + sp[k].at, 8 - sp[k].cut);
     }
   };
   if (AHEAD && blockIdx.x < a.rows) load(blockIdx.x);
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(AHEAD ? 512 : 1024) void norm_bwd_block_kernel(Norm
     float xh[K][8], g[K][8], s1, s2;
     Keep8 m[K];
     const float rstd = in.rstd;
-    bwd_row<TX, TR, RES, K, true, ODD>(a, key, in, sp, false, row, lanes, tl, wlds, xh, g, m, dw, db, s1, s2);
+    bwd_row<TX, TR, RES, K, true, MODE>(a, key, in, sp, false, row, lanes, tl, wlds, xh, g, m, dw, db, s1, s2);
     if (AHEAD && row + gridDim.x < a.rows) load(row + gridDim.x);
     // one barrier a row: the next row writes the other half, and the one after it finds every thread past this row's reads
     s1 = wave64_sum(s1);
@@ -301,37 +301,46 @@ static int norm_parts(long long rows, long long cols, bool lean) {
 }
 
 uint64_t norm_workspace_bytes(long long rows, long long cols) {
-  const int parts = cols < kNormRowMin || cols > kNormRowMax ? norm_wide_parts(rows, cols) : std::max(norm_parts(rows, cols, false), norm_parts(rows, cols, true));
+  const int parts = cols > kNormRowMax ? norm_wide_parts(rows, cols) : std::max(norm_parts(rows, cols, false), norm_parts(rows, cols, true));
   return (uint64_t)parts * 2 * (uint64_t)cols * sizeof(float);
 }
 
-template <class TX, class TR, int RES, bool ODD> static int backward_rows(const NormArgs& a, hipStream_t s) {
+template <class TX, class TR, int RES, LoadMode MODE> static int backward_rows(const NormArgs& a, hipStream_t s) {
   constexpr bool lean = RES == 0 && sizeof(TX) == 2;
   const NormShape sh = bwd_shape(a.cols, lean);
   const int grid = norm_parts(a.rows, a.cols, lean);
   const size_t lds = (size_t)sh.threads * sh.k * 8 * sizeof(float);
-  if (sh.block && sh.k == 4) norm_bwd_block_kernel<TX, TR, RES, lean ? 4 : 2, true, ODD><<<grid, sh.threads, lds, s>>>(a);
-  else if (sh.block && sh.threads <= 512) norm_bwd_block_kernel<TX, TR, RES, 2, true, ODD><<<grid, sh.threads, lds, s>>>(a);
-  else if (sh.block) norm_bwd_block_kernel<TX, TR, RES, 2, false, ODD><<<grid, sh.threads, lds, s>>>(a);
-  else if (sh.k == 1) norm_bwd_kernel<TX, TR, RES, 1, ODD><<<grid, 256, 0, s>>>(a, sh.shift);
-  else if (sh.k == 2) norm_bwd_kernel<TX, TR, RES, 2, ODD><<<grid, 256, 0, s>>>(a, sh.shift);
-  else if (sh.k == 3) norm_bwd_kernel<TX, TR, RES, 3, ODD><<<grid, 256, 0, s>>>(a, sh.shift);
-  else norm_bwd_kernel<TX, TR, RES, 4, ODD><<<grid, 256, 0, s>>>(a, sh.shift);
+  if (sh.block && sh.k == 4) norm_bwd_block_kernel<TX, TR, RES, lean ? 4 : 2, true, MODE><<<grid, sh.threads, lds, s>>>(a);
+  else if (sh.block && sh.threads <= 512) norm_bwd_block_kernel<TX, TR, RES, 2, true, MODE><<<grid, sh.threads, lds, s>>>(a);
+  else if (sh.block) norm_bwd_block_kernel<TX, TR, RES, 2, false, MODE><<<grid, sh.threads, lds, s>>>(a);
+  else if (sh.k == 1) norm_bwd_kernel<TX, TR, RES, 1, MODE><<<grid, 256, 0, s>>>(a, sh.shift);
+  else if (sh.k == 2) norm_bwd_kernel<TX, TR, RES, 2, MODE><<<grid, 256, 0, s>>>(a, sh.shift);
+  else if (sh.k == 3) norm_bwd_kernel<TX, TR, RES, 3, MODE><<<grid, 256, 0, s>>>(a, sh.shift);
+  else norm_bwd_kernel<TX, TR, RES, 4, MODE><<<grid, 256, 0, s>>>(a, sh.shift);
+  if (check_launch("norm_backward")) return -1;
+  if (grid > 1 && (a.dweight != nullptr || a.dbias != nullptr)) return norm_finish(a, grid, s);
+  return 0;
+}
+
+template <class TX, class TR, int RES> static int backward_short(const NormArgs& a, hipStream_t s) {
+  const int grid = norm_parts(a.rows, a.cols, false);
+  norm_bwd_kernel<TX, TR, RES, 1, kShort><<<grid, 256, 0, s>>>(a, bwd_shape(a.cols, false).shift);
   if (check_launch("norm_backward")) return -1;
   if (grid > 1 && (a.dweight != nullptr || a.dbias != nullptr)) return norm_finish(a, grid, s);
   return 0;
 }
 
 template <class TX, class TR, int RES> static int backward(const NormArgs& a, hipStream_t s) {
-  constexpr bool can = RES == 0 && sizeof(TX) == 2;      // (norm.hpp, odd_rows)
-  if (can && (odd_rows(a.x, a.ld_x) || odd_rows(a.dy, a.ld_dy))) return backward_rows<TX, TR, RES, can>(a, s);
-  return backward_rows<TX, TR, RES, false>(a, s);
+  constexpr LoadMode odd = sizeof(TX) == 2 ? kOdd : kPlain;
+  if (a.cols < 8) return backward_short<TX, TR, RES>(a, s);
+  if (odd == kOdd && (odd_rows<TX>(a.x, a.ld_x) || odd_rows<TR>(a.dy, a.ld_dy) || (RES && odd_rows<TR>(a.residual, a.ld_r)))) return backward_rows<TX, TR, RES, odd>(a, s);
+  return backward_rows<TX, TR, RES, kPlain>(a, s);
 }
 
 int norm_backward(const NormArgs& a, hipStream_t stream) {
   ProfScope prof("norm_backward", stream, 14.0 * a.rows * a.cols,
                  (double)a.rows * a.cols * (2.0 * elem_size(a.x_type) + elem_size(a.y_type) * (a.residual ? 3.0 : 1.0)));
-  if (a.cols < kNormRowMin || a.cols > kNormRowMax) return norm_wide_backward(a, stream);
+  if (a.cols > kNormRowMax) return norm_wide_backward(a, stream);
   NORM_DISPATCH(backward, a, stream);
 }
 

@@ -11,7 +11,7 @@ template <class TX, class TR, int K> struct FwdRow {
 };
 
 // z of a loaded row, its sum in s
-template <class TX, class TR, int RES, int K, bool BLK, bool ODD>
+template <class TX, class TR, int RES, int K, bool BLK, LoadMode MODE>
 __device__ __forceinline__ float join_row(const NormArgs& a, const DropKey& key, FwdRow<TX, TR, K>& in, const Span (&sp)[K], long long row,
                                           int lanes, int tl, float (&z)[K][8]) {
   float s = 0.0f;
@@ -19,8 +19,8 @@ __device__ __forceinline__ float join_row(const NormArgs& a, const DropKey& key,
   if (RES && a.drop.on) keep_row<K, BLK>(m, (uint64_t)(row * a.cols), key, a.drop.tm1, (int)a.cols, lanes, tl);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    in.x[k].template cut<ODD>(sp[k].cut);
-    if (RES) in.r[k].template cut<ODD>(sp[k].cut);
+    in.x[k].template cut<MODE>(sp[k].cut);
+    if (RES) in.r[k].template cut<MODE>(sp[k].cut);
     if (RES && a.drop.on) {
       const uint32_t limit = keep_limit(a.drop.tm1);
 #pragma unroll
@@ -60,7 +60,7 @@ template <class TR> __device__ __forceinline__ void put_y(TR* y, float (&z)[8], 
 
 // Rows of up to 2048 columns.  U rows a team are loaded before the first is used, and a workgroup ends after them: a grid in row order
 // keeps the whole chip on neighbouring pages.
-template <class TX, class TR, int RES, int K, int U, bool ODD>
+template <class TX, class TR, int RES, int K, int U, LoadMode MODE>
 __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift) {
   const int lanes = 1 << shift, tl = threadIdx.x & (lanes - 1), team = threadIdx.x >> shift, teams = 256 >> shift, cols = (int)a.cols;
   const float inv = 1.0f / (float)cols;
@@ -68,7 +68,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift) {
   if (RES) key = drop_key(a.drop);
   Span sp[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) sp[k] = Span((k * lanes + tl) * 8, cols);
+  for (int k = 0; k < K; ++k) sp[k] = Span::of<MODE>((k * lanes + tl) * 8, cols, k == K - 1);
   const long long base = (long long)blockIdx.x * (teams * U);
   const int last = (int)min((long long)(teams * U), a.rows - base) - 1;          // of this workgroup's rows
   const TX* px = reinterpret_cast<const TX*>(a.x) + base * a.ld_x;
@@ -80,21 +80,21 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift) {
     const uint32_t r = min(u * teams + team, last);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      in[u].x[k].template load<ODD>(px + row_at(r, (uint32_t)a.ld_x, sp[k].at));
-      if (RES) in[u].r[k].template load<ODD>(pr + row_at(r, (uint32_t)a.ld_r, sp[k].at));
+      in[u].x[k].template load<MODE>(px + row_at(r, (uint32_t)a.ld_x, sp[k].at), 8 - sp[k].cut);
+      if (RES) in[u].r[k].template load<MODE>(pr + row_at(r, (uint32_t)a.ld_r, sp[k].at), 8 - sp[k].cut);
     }
   }
   float w[K][8], b[K][8];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    load_param<TX>(a.weight, a.p_f32, sp[k], 1.0f, w[k]);
-    load_param<TX>(a.bias, a.p_f32, sp[k], 0.0f, b[k]);
+    load_param<TX, MODE == kShort ? kShort : kPlain>(a.weight, a.p_f32, sp[k], 1.0f, w[k]);
+    load_param<TX, MODE == kShort ? kShort : kPlain>(a.bias, a.p_f32, sp[k], 0.0f, b[k]);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int r = u * teams + team;
     float z[K][8];
-    const float mean = lanes_sum(join_row<TX, TR, RES, K, false, ODD>(a, key, in[u], sp, base + r, lanes, tl, z), shift) * inv;
+    const float mean = lanes_sum(join_row<TX, TR, RES, K, false, MODE>(a, key, in[u], sp, base + r, lanes, tl, z), shift) * inv;
     const float rstd = rsqrt_newton(lanes_sum(deviate<K>(z, mean, sp), shift) * inv + a.eps);
     if (r > last) continue;
     if (tl == 0 && a.mean != nullptr) {
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift) {
 
 // Rows of a workgroup.  The next row's loads are issued when this row has become z, so they pass behind its two sums and its stores: with
 // 512 or 1024 threads a row only one or two rows are on a CU, and without that its memory was idle half of the time.
-template <class TX, class TR, int RES, int K, bool ODD>
+template <class TX, class TR, int RES, int K, LoadMode MODE>
 __global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
   __shared__ float sm[2][16];
   const int lanes = blockDim.x, tl = threadIdx.x, cols = (int)a.cols;
@@ -118,27 +118,27 @@ __global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
   if (RES) key = drop_key(a.drop);
   Span sp[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) sp[k] = Span((k * lanes + tl) * 8, cols);
+  for (int k = 0; k < K; ++k) sp[k] = Span::of<MODE>((k * lanes + tl) * 8, cols, k == K - 1);
   FwdRow<TX, TR, K> in;
   const auto load = [&](long long row) {
     const TX* px = reinterpret_cast<const TX*>(a.x) + row * a.ld_x;
     const TR* pr = reinterpret_cast<const TR*>(a.residual) + row * a.ld_r;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      in.x[k].template load<ODD>(px + sp[k].at);
-      if (RES) in.r[k].template load<ODD>(pr + sp[k].at);
+      in.x[k].template load<MODE>(px + sp[k].at, 8 - sp[k].cut);
+      if (RES) in.r[k].template load<MODE>(pr + sp[k].at, 8 - sp[k].cut);
     }
   };
   float w[K][8], b[K][8];
   load(blockIdx.x);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    load_param<TX>(a.weight, a.p_f32, sp[k], 1.0f, w[k]);
-    load_param<TX>(a.bias, a.p_f32, sp[k], 0.0f, b[k]);
+    load_param<TX, MODE == kShort ? kShort : kPlain>(a.weight, a.p_f32, sp[k], 1.0f, w[k]);
+    load_param<TX, MODE == kShort ? kShort : kPlain>(a.bias, a.p_f32, sp[k], 0.0f, b[k]);
   }
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     float z[K][8];
-    const float s = join_row<TX, TR, RES, K, true, ODD>(a, key, in, sp, row, lanes, tl, z);
+    const float s = join_row<TX, TR, RES, K, true, MODE>(a, key, in, sp, row, lanes, tl, z);
     if (row + gridDim.x < a.rows) load(row + gridDim.x);
     const float mean = block_sum(s, sm[0]) * inv;
     const float rstd = rsqrt_newton(block_sum(deviate<K>(z, mean, sp), sm[1]) * inv + a.eps);
@@ -159,37 +159,40 @@ constexpr long long kManyGroups = 2048;
 // Chunks that a wave may hold: the join's four a lane leave two waves a SIMD (93750 x 1600 bf16: 218 us, 181 in a workgroup), three do not
 // (97656 x 1536: 156 us, 179 in a workgroup).
 template <int RES> constexpr int wave_chunks() { return RES ? 192 : 256; }
-template <class TX, class TR, int RES, int K, int U, bool ODD> static int wave_forward(const NormArgs& a, const NormShape& sh, hipStream_t s) {
+template <class TX, class TR, int RES, int K, int U, LoadMode MODE> static int wave_forward(const NormArgs& a, const NormShape& sh, hipStream_t s) {
   const long long per = (long long)sh.teams() * U, grid = (a.rows + per - 1) / per;
   LBM_REQUIRE(grid < (1ll << 31), "norm_forward: %lld rows are more than a grid holds", a.rows);
-  norm_fwd_kernel<TX, TR, RES, K, U, ODD><<<(unsigned)grid, 256, 0, s>>>(a, sh.shift);
+  norm_fwd_kernel<TX, TR, RES, K, U, MODE><<<(unsigned)grid, 256, 0, s>>>(a, sh.shift);
   return check_launch("norm_forward");
 }
-template <class TX, class TR, int RES, bool ODD> static int forward_rows(const NormArgs& a, hipStream_t s) {
+template <class TX, class TR, int RES, LoadMode MODE> static int forward_rows(const NormArgs& a, hipStream_t s) {
   const NormShape sh = norm_shape(a.cols, wave_chunks<RES>());
   if (sh.block) {
     const long long most = 256 * (1024 / sh.threads);      // what is resident at once (16 waves a CU), a whole number a CU
-    norm_fwd_block_kernel<TX, TR, RES, 2, ODD><<<(unsigned)(a.rows < most ? a.rows : most), sh.threads, 0, s>>>(a);
+    norm_fwd_block_kernel<TX, TR, RES, 2, MODE><<<(unsigned)(a.rows < most ? a.rows : most), sh.threads, 0, s>>>(a);
     return check_launch("norm_forward");
   }
   constexpr int U1 = RES ? 2 : 4, U2 = RES ? 1 : 2;
-  if (sh.k == 4) return wave_forward<TX, TR, RES, 4, 1, ODD>(a, sh, s);
+  if (sh.k == 4) return wave_forward<TX, TR, RES, 4, 1, MODE>(a, sh, s);
   const bool many = a.rows >= (long long)sh.teams() * (sh.k == 1 ? U1 : U2) * kManyGroups;
-  if (sh.k == 1) return many ? wave_forward<TX, TR, RES, 1, U1, ODD>(a, sh, s) : wave_forward<TX, TR, RES, 1, 1, ODD>(a, sh, s);
-  if (sh.k == 2) return many ? wave_forward<TX, TR, RES, 2, U2, ODD>(a, sh, s) : wave_forward<TX, TR, RES, 2, 1, ODD>(a, sh, s);
-  return many ? wave_forward<TX, TR, RES, 3, U2, ODD>(a, sh, s) : wave_forward<TX, TR, RES, 3, 1, ODD>(a, sh, s);
+  if (sh.k == 1) return many ? wave_forward<TX, TR, RES, 1, U1, MODE>(a, sh, s) : wave_forward<TX, TR, RES, 1, 1, MODE>(a, sh, s);
+  if (sh.k == 2) return many ? wave_forward<TX, TR, RES, 2, U2, MODE>(a, sh, s) : wave_forward<TX, TR, RES, 2, 1, MODE>(a, sh, s);
+  return many ? wave_forward<TX, TR, RES, 3, U2, MODE>(a, sh, s) : wave_forward<TX, TR, RES, 3, 1, MODE>(a, sh, s);
 }
 template <class TX, class TR, int RES> static int forward(const NormArgs& a, hipStream_t s) {
-  constexpr bool can = RES == 0 && sizeof(TX) == 2;      // (norm.hpp, odd_rows)
-  if (can && odd_rows(a.x, a.ld_x)) return forward_rows<TX, TR, RES, can>(a, s);
-  return forward_rows<TX, TR, RES, false>(a, s);
+  constexpr LoadMode odd = sizeof(TX) == 2 ? kOdd : kPlain;
+  if (a.cols < 8) return wave_forward<TX, TR, RES, 1, 1, kShort>(a, norm_shape(a.cols, 1), s);
+  // (the join's two chunks a lane are the exception: 146914 x 1021 bf16 184 us with plain loads, 201 dword by dword)
+  const NormShape sh = norm_shape(a.cols, wave_chunks<RES>());
+  if (odd == kOdd && (odd_rows<TX>(a.x, a.ld_x) || (RES && odd_rows<TR>(a.residual, a.ld_r))) && !(RES && !sh.block && sh.k == 2)) return forward_rows<TX, TR, RES, odd>(a, s);
+  return forward_rows<TX, TR, RES, kPlain>(a, s);
 }
 
 int norm_forward(const NormArgs& a, hipStream_t stream) {
   if (a.rows == 0) return 0;
   ProfScope prof("norm_forward", stream, 8.0 * a.rows * a.cols,
                  (double)a.rows * a.cols * (elem_size(a.x_type) + elem_size(a.y_type) * (a.residual ? 2.0 : 1.0)));
-  if (a.cols < kNormRowMin || a.cols > kNormRowMax) return norm_wide_forward(a, stream);
+  if (a.cols > kNormRowMax) return norm_wide_forward(a, stream);
   NORM_DISPATCH(forward, a, stream);
 }
 

@@ -121,12 +121,13 @@ __device__ __forceinline__ Keep8 keep8(uint64_t e, const DropKey& k, uint32_t tm
 
 // ---- eight consecutive elements of a row ---------------------------------------------------------------------------
 // One 16-byte access (two for fp32): gfx950 serves unaligned global accesses, at full rate where they start at a dword.
-//   load           eight elements; near a row's end the caller reads earlier ones and cuts (below).  ODD: half-precision rows that may start
+//   load           eight elements; near a row's end the caller reads earlier ones and cuts (below).  kOdd: half-precision rows that may start
 //                  in the middle of a dword (6001 columns: 3.7 TB/s instead of 5.2 in the backward pass) are read from the dwords
-//                  that hold them and shifted in cut; no dword without one of the eight is touched
-//   load_some      the first nv of eight, element by element
-//   cut(s)         drops the first s elements and fills up with zeros (s = 8: all zeros)
+//                  that hold them and shifted in cut; no dword without one of the eight is touched.  kShort: rows of n < 8 elements
+//   load_some      the first nv of eight, element by element, and zeros
+//   cut(s)         drops the first s elements and fills up with zeros (s = 8: all zeros); kShort: nothing but s = 8
 //   store(p, nv)   the first nv of eight
+enum LoadMode { kPlain, kOdd, kShort };
 template <class T> struct Vec8;
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
 typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
@@ -140,7 +141,11 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 template <> struct Vec8<float> {
   u32x4 a, b;
-  template <bool ODD = false> __device__ __forceinline__ void load(const float* p) {
+  template <LoadMode MODE = kPlain> __device__ __forceinline__ void load(const float* p, int n = 8) {
+    if (MODE == kShort) {
+      load_some(p, n);
+      return;
+    }
     a = *reinterpret_cast<const u32x4_a4*>(p);
     b = *reinterpret_cast<const u32x4_a4*>(p + 4);
   }
@@ -154,7 +159,11 @@ template <> struct Vec8<float> {
         else b[j & 3] = w;
       }
   }
-  template <bool ODD = false> __device__ __forceinline__ void cut(int s) {
+  template <LoadMode MODE = kPlain> __device__ __forceinline__ void cut(int s) {
+    if (MODE == kShort) {
+      if (s == 8) a = b = u32x4{0, 0, 0, 0};
+      return;
+    }
     if (s == 0) return;
     if (s & 4) { a = b; b = u32x4{0, 0, 0, 0}; }
     if (s & 2) { a = u32x4{a[2], a[3], b[0], b[1]}; b = u32x4{b[2], b[3], 0, 0}; }
@@ -184,9 +193,11 @@ template <> struct Vec8<float> {
 };
 struct Vec8Half {       // f16 and bf16: eight elements in four words
   u32x4 a;
-  uint32_t fifth, shift;          // ODD only: the dword behind the four, and 0 or 16
-  template <bool ODD = false> __device__ __forceinline__ void load(const void* p) {
-    if (ODD) {
+  uint32_t fifth, shift;          // kOdd only: the dword behind the four, and 0 or 16
+  template <LoadMode MODE = kPlain> __device__ __forceinline__ void load(const void* p, int n = 8) {
+    if (MODE == kShort) {
+      load_some(p, n);
+    } else if (MODE == kOdd) {
       const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 2u;
       const char* q = reinterpret_cast<const char*>(p) - off;
       a = *reinterpret_cast<const u32x4_a4*>(q);
@@ -203,8 +214,12 @@ struct Vec8Half {       // f16 and bf16: eight elements in four words
     for (int j = 0; j < 8; ++j)
       if (j < nv) a[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
   }
-  template <bool ODD = false> __device__ __forceinline__ void cut(int s) {
-    if (ODD)
+  template <LoadMode MODE = kPlain> __device__ __forceinline__ void cut(int s) {
+    if (MODE == kShort) {
+      if (s == 8) a = u32x4{0, 0, 0, 0};
+      return;
+    }
+    if (MODE == kOdd)
       a = u32x4{__builtin_amdgcn_alignbit(a[1], a[0], shift), __builtin_amdgcn_alignbit(a[2], a[1], shift), __builtin_amdgcn_alignbit(a[3], a[2], shift),
                 __builtin_amdgcn_alignbit(fifth, a[3], shift)};
     if (s == 0) return;

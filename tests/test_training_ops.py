@@ -314,6 +314,19 @@ def test_norm_numbers_of_rows(rows, cols):
 
 
 @gpu
+@pytest.mark.parametrize("cols", [1, 2, 3, 4, 5, 6, 7])
+def test_norm_short_rows(cols):
+    """Rows of fewer than eight elements, many of them, dense and apart, every type."""
+    for k, types in enumerate(TYPES):
+        rows = (1, 255, 257, 4000)[k % 4]
+        o = operands((rows, cols), *types, ("both", "weight", "none")[k % 3], seed=cols * 10 + k)
+        check(o, p=0.3, seed=k, offset=cols)
+        wide = torch.full((rows, cols + 3), float("nan"), device="cuda", dtype=types[0])
+        wide[:, 1:1 + cols] = o["x"]
+        check(o, p=0.3, seed=k, offset=cols, x_view=wide[:, 1:1 + cols])
+
+
+@gpu
 @pytest.mark.parametrize("affine", ["both", "weight", "bias", "none"])
 def test_norm_shapes_and_strides(affine):
     g = torch.Generator("cuda").manual_seed(2)
