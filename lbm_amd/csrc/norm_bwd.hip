@@ -109,10 +109,12 @@ __device__ __forceinline__ void bwd_put(const NormArgs& a, const Span (&sp)[K], 
 }
 
 // Rows of lanes of a wave.  The next row's loads are issued when this row has become xhat and g, and pass behind its sums and stores.
+// Eight waves a workgroup, one workgroup a CU: half the partial sums of four waves and two (150000 x 1024 join 315 -> 295 us, 16320 x 257 16.4 -> 15.1).
+constexpr int kBwdThreads = 512, kBwdWaves = kBwdThreads / 64;
 template <class TX, class TR, int RES, int K, LoadMode MODE>
-__global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a, int shift) {
-  __shared__ __align__(16) float red[4 * 512 * K];         // the weights (K > 1); at the end one column sum of every wave
-  const int lanes = 1 << shift, tl = threadIdx.x & (lanes - 1), team = threadIdx.x >> shift, teams = 256 >> shift, cols = (int)a.cols;
+__global__ __launch_bounds__(kBwdThreads) void norm_bwd_kernel(NormArgs a, int shift) {
+  __shared__ __align__(16) float red[kBwdWaves * 512 * K];         // the weights (K > 1); at the end one column sum of every wave
+  const int lanes = 1 << shift, tl = threadIdx.x & (lanes - 1), team = threadIdx.x >> shift, teams = kBwdThreads >> shift, cols = (int)a.cols;
   const float inv = 1.0f / (float)cols;
   DropKey key{};
   if (RES) key = drop_key(a.drop);
@@ -157,7 +159,7 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a, int shift) {
     if (row < a.rows) bwd_put<TX, TR, RES, K>(a, sp, row * a.cols, lanes, tl, c1, c2, rstd, xh, g, m);
   }
   if (a.dweight == nullptr && a.dbias == nullptr) return;
-  // the teams of a wave, then the four waves
+  // the teams of a wave, then the waves
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     float(&acc)[K][8] = which == 0 ? dw : db;
@@ -174,8 +176,12 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a, int shift) {
         for (int j = 0; j < 8; ++j) red[(threadIdx.x >> 6) * (512 * K) + (k * lanes + tl) * 8 + j] = acc[k][j];
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < cols; c += 256)
-      put_part<TX>(a, which, c, (red[c] + red[512 * K + c]) + (red[2 * 512 * K + c] + red[3 * 512 * K + c]));
+    for (int c = threadIdx.x; c < cols; c += kBwdThreads) {
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kBwdWaves; ++i) s += red[i * (512 * K) + c];
+      put_part<TX>(a, which, c, s);
+    }
   }
 }
 
@@ -284,19 +290,20 @@ int norm_finish(const NormArgs& a, int parts, hipStream_t s) {
 // precision without a residual), else 1024 threads that load a row at a time.
 static NormShape bwd_shape(long long cols, bool lean) {
   const int chunks = (int)((cols + 7) / 8);
-  if (chunks <= 192) return norm_shape(cols, 192);
-  NormShape s{chunks > 1024 && lean ? 4 : 2, 0, 0, true};
+  NormShape s = norm_shape(cols, 192);
+  s.threads = kBwdThreads;
+  if (chunks <= 192) return s;
+  s = NormShape{chunks > 1024 && lean ? 4 : 2, 0, 0, true};
   s.threads = (chunks + 64 * s.k - 1) / (64 * s.k) * 64;
   return s;
 }
 // workgroups = partial sums: what is resident at once, a whole number a CU (the sums a workgroup keeps make the launch persistent)
 static int norm_parts(long long rows, long long cols, bool lean) {
   const NormShape sh = bwd_shape(cols, lean);
-  int per_cu = 2;
-  if (sh.block) per_cu = sh.threads <= 128 ? 3 : sh.threads <= 256 ? 2 : 1;
-  while (sh.block && per_cu > 1 && rows < 8 * 256 * per_cu) --per_cu;      // a partial sum costs as much traffic as four rows
+  int per_cu = !sh.block ? 1 : sh.threads <= 128 ? 3 : sh.threads <= 256 ? 2 : 1;
+  while (per_cu > 1 && rows < 8 * 256 * per_cu) --per_cu;      // a partial sum costs the traffic of two or three rows
   const long long g = (rows + sh.teams() - 1) / sh.teams();
-  if (g <= (sh.block || sh.k > 1 ? 2 : 4)) return 1;       // a few rounds of one workgroup (32 x 256: 5.3 us) cost less than the second launch (8.4)
+  if (g <= (sh.block || sh.k > 1 ? 2 : 4)) return 1;       // a few rounds of one workgroup (64 x 256: 6.3 us) cost less than the second launch (8.3)
   return (int)std::min(g, 256ll * per_cu);
 }
 
@@ -313,10 +320,10 @@ template <class TX, class TR, int RES, LoadMode MODE> static int backward_rows(c
   if (sh.block && sh.k == 4) norm_bwd_block_kernel<TX, TR, RES, lean ? 4 : 2, true, MODE><<<grid, sh.threads, lds, s>>>(a);
   else if (sh.block && sh.threads <= 512) norm_bwd_block_kernel<TX, TR, RES, 2, true, MODE><<<grid, sh.threads, lds, s>>>(a);
   else if (sh.block) norm_bwd_block_kernel<TX, TR, RES, 2, false, MODE><<<grid, sh.threads, lds, s>>>(a);
-  else if (sh.k == 1) norm_bwd_kernel<TX, TR, RES, 1, MODE><<<grid, 256, 0, s>>>(a, sh.shift);
-  else if (sh.k == 2) norm_bwd_kernel<TX, TR, RES, 2, MODE><<<grid, 256, 0, s>>>(a, sh.shift);
-  else if (sh.k == 3) norm_bwd_kernel<TX, TR, RES, 3, MODE><<<grid, 256, 0, s>>>(a, sh.shift);
-  else norm_bwd_kernel<TX, TR, RES, 4, MODE><<<grid, 256, 0, s>>>(a, sh.shift);
+  else if (sh.k == 1) norm_bwd_kernel<TX, TR, RES, 1, MODE><<<grid, kBwdThreads, 0, s>>>(a, sh.shift);
+  else if (sh.k == 2) norm_bwd_kernel<TX, TR, RES, 2, MODE><<<grid, kBwdThreads, 0, s>>>(a, sh.shift);
+  else if (sh.k == 3) norm_bwd_kernel<TX, TR, RES, 3, MODE><<<grid, kBwdThreads, 0, s>>>(a, sh.shift);
+  else norm_bwd_kernel<TX, TR, RES, 4, MODE><<<grid, kBwdThreads, 0, s>>>(a, sh.shift);
   if (check_launch("norm_backward")) return -1;
   if (grid > 1 && (a.dweight != nullptr || a.dbias != nullptr)) return norm_finish(a, grid, s);
   return 0;
@@ -324,7 +331,7 @@ template <class TX, class TR, int RES, LoadMode MODE> static int backward_rows(c
 
 template <class TX, class TR, int RES> static int backward_short(const NormArgs& a, hipStream_t s) {
   const int grid = norm_parts(a.rows, a.cols, false);
-  norm_bwd_kernel<TX, TR, RES, 1, kShort><<<grid, 256, 0, s>>>(a, bwd_shape(a.cols, false).shift);
+  norm_bwd_kernel<TX, TR, RES, 1, kShort><<<grid, kBwdThreads, 0, s>>>(a, bwd_shape(a.cols, false).shift);
   if (check_launch("norm_backward")) return -1;
   if (grid > 1 && (a.dweight != nullptr || a.dbias != nullptr)) return norm_finish(a, grid, s);
   return 0;
