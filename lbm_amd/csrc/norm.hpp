@@ -78,7 +78,8 @@ template <class TX, LoadMode MODE> __device__ __forceinline__ void load_param(co
 }
 // element offset of row r (below 2^32) at a stride below 2^31: one multiply
 __device__ __forceinline__ uint64_t row_at(uint32_t r, uint32_t ld, int c) { return (uint64_t)r * ld + (uint32_t)c; }
-// 1 / sqrt(v): v_rsq_f32 (1 ulp) and a Newton step in place of the correctly rounded square root and division (~25 instructions a row)
+// 1 / sqrt(v): v_rsq_f32 (1 ulp) and a Newton step in place of the correctly rounded square root and division (~25 instructions a row).  A variance
+// beyond the range (infinite) gives NaN: no row of zeros that looks like a result.
 __device__ __forceinline__ float rsqrt_newton(float v) {
   const float r = __builtin_amdgcn_rsqf(v);
   const float e = fmaf(-v * r, r, 1.0f);

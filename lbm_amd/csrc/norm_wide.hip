@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) s += j < nv ? (z[j] - mean) * (z[j] - mean) : 0.0f;
     }
-    const float rstd = 1.0f / sqrtf(block_sum(s, sm[1]) / (float)a.cols + a.eps);
+    const float rstd = rsqrt_newton(block_sum(s, sm[1]) / (float)a.cols + a.eps);
     if (threadIdx.x == 0 && a.mean != nullptr) {
       a.mean[row] = mean;
       a.rstd[row] = rstd;

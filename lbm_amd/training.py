@@ -34,7 +34,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
     x (..., D): rows of the last dimension at one stride are read where they lie (a slice of a merged projection), any other
     layout is copied first.  weight / bias (D,): x's type or float32, both the same; either may be None.  The result is dense.
-    Squared deviations beyond fp32's range (3.4e38) are outside the domain."""
+    A row whose squared deviations add up beyond fp32's range (3.4e38) gives NaN."""
     return hip.ops().norm(x, None, weight, bias, eps, 0.0, 0, None, 0)
 
 

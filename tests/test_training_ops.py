@@ -376,6 +376,36 @@ def test_norm_rows_of_special_values():
 
 
 @gpu
+@pytest.mark.parametrize("cols", [5, 256, 257, 5000, 17000])
+def test_norm_rows_beyond_the_range_of_fp32_are_nan(cols):
+    x = torch.randn(6, cols, device="cuda", generator=torch.Generator("cuda").manual_seed(8))
+    clean = layer_norm(x)
+    x[2] *= 1e25
+    y = layer_norm(x)
+    rest = [0, 1, 3, 4, 5]
+    assert bool(y[2].isnan().all()) and torch.equal(y[rest], clean[rest])
+
+
+@gpu
+@pytest.mark.parametrize("cols", [256, 257])
+def test_norm_beyond_32_bit_indexes(cols):
+    """2.2e9 elements, 4.3 GB a tensor: rows at the far end and around 2^31 elements and bytes against the oracle."""
+    rows, p, seed, offset = 2_200_000_000 // cols, 0.3, 99, 5
+    g = torch.Generator("cuda").manual_seed(9)
+    x, r, dy = (torch.empty(rows, cols, device="cuda", dtype=F16).normal_(generator=g) for _ in range(3))
+    w, b = (torch.randn(cols, device="cuda", generator=g) for _ in range(2))
+    y, mean, rstd = hip.norm_forward(x, w, b, 1e-5, r, p, seed, offset, want_stats=True)
+    dx, dres, _, _ = hip.norm_backward(dy, x, mean, rstd, w, b, 1e-5, r, p, seed, offset, want=(True, True, False, False))
+    for first in (0, 2 ** 30 // cols - 3, 2 ** 31 // cols - 3, rows - 6):
+        part = slice(first, first + 6)
+        factor = ref.keep((6, cols), p, seed, offset, first=first * cols).double() * ref.scale(p)
+        want = ref.norm(x[part], w, b, 1e-5, r[part], factor, dy[part])
+        tol = bounds(want, 1e-5, F16, F16, F32, ref.scale(p))
+        for name, got in (("y", y), ("dx", dx), ("dresidual", dres)):
+            within(got[part], want[name], tol[name], name)
+
+
+@gpu
 def test_join_drops_non_finite_values():
     x = torch.randn(16, 256, device="cuda", generator=torch.Generator("cuda").manual_seed(5))
     m = ref.keep((16, 256), 0.5, 21, 2).cuda()
