@@ -17,7 +17,7 @@ int make_drop(double p, uint64_t seed, const void* seed_ptr, uint64_t offset, Dr
 }
 
 // A thread takes one chunk of eight elements, which is one block of the generator, and ends: bound by HBM (67108864 bf16 46 us, 5.8 TB/s;
-// 150994944 bf16 99 us, 6.1; fp32 207 us, 5.8: its chunk is two 16-byte accesses 32 bytes apart).  A grid that strides over the chunks
+// 150994944 bf16 99 us, 6.1; fp32 207 us, 5.8: its lanes lie 32 bytes apart).  A grid that strides over the chunks
 // instead reached 4.4 - 5.0 TB/s; the ten rounds are hidden behind the memory (0, 7 or 10 of them: 345, 347, 342 us a GiB).
 template <class T>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* x, T* y, long long n, DropArgs d) {
