@@ -95,7 +95,8 @@ int lbm_hip_dropout(const void* x, void* y, int64_t n, int32_t type, double p, u
                     lbm_stream_t stream);
 
 /* z = x (residual == NULL) or residual + dropout(x);  y = (z - mean(z)) * rstd * weight + bias per row,
- * rstd = 1 / sqrt(mean((z - mean)^2) + eps).  Statistics and sums are fp32.  Types: x and dx x_type; residual, y, dy and dresidual
+ * rstd = 1 / sqrt(mean((z - mean)^2) + eps).  Statistics and sums are fp32; the forward pass corrects its mean by the mean of the
+ * deviations from it, so a row far from zero loses nothing of its spread; the backward pass takes z from the stored mean, which is rounded to fp32.  Types: x and dx x_type; residual, y, dy and dresidual
  * res_type (= x_type, or LBM_TYPE_F32: half-precision products beside an fp32 residual stream; without a residual = x_type);
  * weight, bias and their gradients param_type (= x_type or LBM_TYPE_F32), either may be NULL.  Element strides between rows:
  * ld_x, ld_residual, ld_dy (>= cols, < 2^31); outputs are dense and overlap no input.  1 <= cols <= 2^28.

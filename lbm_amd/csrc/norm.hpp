@@ -86,6 +86,22 @@ __device__ __forceinline__ float rsqrt_newton(float v) {
   return fmaf(0.5f * r, e, r);
 }
 
+// The first mean m of a row is its sum times 1 / cols in fp32, off by some roundings of m: of no account beside the spread unless the row lies far from
+// zero (1000 columns of 1000.1: 0.02 after the division by sqrt(eps)).  The second pass therefore sums the deviations z - m themselves beside their squares:
+//   d = mean(z - m): the mean is m + d;   var = mean((z - m)^2) - d^2,   z - mean = (z - m) - d
+// What is left grows with the spread and with e^2 |m|.  Both sums are exact enough for d^2 as long as the variance is not far below it; where it is
+// (a constant row), the difference is rounding noise and 2^-18 of the squares stands for it, so that no eps makes a result of that noise.
+__device__ __forceinline__ float norm_variance(float squares, float d) {
+  const float v = fmaf(-d, d, squares), least = squares * 0x1p-18f;
+  return v > least ? v : least;              // NaN and infinity come through `least`
+}
+
+// a * b rounded by itself: contracted into the subtractions, m would be another number in z - m than in m + d
+__device__ __forceinline__ float product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
 __device__ __forceinline__ float lane16_sum(float v) {     // v + the value 16 lanes away (lane ^ 16)
   const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
   const unsigned r0 = r[0], r1 = r[1];

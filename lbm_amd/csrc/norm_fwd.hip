@@ -1,6 +1,6 @@
 // Layer normalisation with the row in registers: y = (z - mean) rstd w + b, z = x or residual + dropout(x).
-// One sweep over memory: a team of threads (norm.hpp) loads its row, sums it, sums the squared deviations from that mean (the two-pass
-// form: no cancellation however large the mean) and writes y.  Bound by HBM: x (and residual) in, y out.
+// One sweep over memory: a team of threads (norm.hpp) loads its row, sums it, sums the deviations from that mean and their squares (the
+// two-pass form; the deviations' own mean corrects the first one, norm.hpp) and writes y.  Bound by HBM: x (and residual) in, y out.
 #include "norm.hpp"
 
 namespace lbm {
@@ -34,9 +34,9 @@ __device__ __forceinline__ float join_row(const NormArgs& a, const DropKey& key,
   }
   return s;
 }
-// z -= mean; the sum of its squares over the elements that exist
-template <int K> __device__ __forceinline__ float deviate(float (&z)[K][8], float mean, const Span (&sp)[K]) {
-  float s = 0.0f;
+// z -= mean; the sum of its squares and its own sum d over the elements that exist
+template <int K> __device__ __forceinline__ float deviate(float (&z)[K][8], float mean, const Span (&sp)[K], float& d) {
+  float s = d = 0.0f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -46,13 +46,17 @@ template <int K> __device__ __forceinline__ float deviate(float (&z)[K][8], floa
       for (int j = 0; j < 8; ++j) z[k][j] = j < 8 - sp[k].cut ? z[k][j] : 0.0f;
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s = fmaf(z[k][j], z[k][j], s);
+    for (int j = 0; j < 8; ++j) {
+      s = fmaf(z[k][j], z[k][j], s);
+      d += z[k][j];
+    }
   }
   return s;
 }
-template <class TR> __device__ __forceinline__ void put_y(TR* y, float (&z)[8], float rstd, const float (&w)[8], const float (&b)[8], int cut) {
+// dr = d rstd: (z - d) rstd in one instruction, off by e |d| rstd, and d is some e |mean| itself
+template <class TR> __device__ __forceinline__ void put_y(TR* y, float (&z)[8], float dr, float rstd, const float (&w)[8], const float (&b)[8], int cut) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) z[j] = fmaf(z[j] * rstd, w[j], b[j]);
+  for (int j = 0; j < 8; ++j) z[j] = fmaf(fmaf(z[j], rstd, -dr), w[j], b[j]);
   Vec8<TR> o;
   o.set(z);
   o.store(y, 8 - cut);
@@ -95,16 +99,19 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift) {
   for (int u = 0; u < U; ++u) {
     const int r = u * teams + team;
     float z[K][8];
-    const float mean = lanes_sum(join_row<TX, TR, RES, K, false, MODE>(a, key, in[u], sp, base + r, lanes, tl, z), shift) * inv;
-    const float rstd = rsqrt_newton(lanes_sum(deviate<K>(z, mean, sp), shift) * inv + a.eps);
+    const float mean = product(lanes_sum(join_row<TX, TR, RES, K, false, MODE>(a, key, in[u], sp, base + r, lanes, tl, z), shift), inv);
+    float d;
+    const float s = deviate<K>(z, mean, sp, d);
+    d = product(lanes_sum(d, shift), inv);
+    const float rstd = rsqrt_newton(norm_variance(lanes_sum(s, shift) * inv, d) + a.eps);
     if (r > last) continue;
     if (tl == 0 && a.mean != nullptr) {
-      a.mean[base + r] = mean;
+      a.mean[base + r] = mean + d;
       a.rstd[base + r] = rstd;
     }
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      if (sp[k].cut < 8) put_y<TR>(py + row_at(r, (uint32_t)cols, (k * lanes + tl) * 8), z[k], rstd, w[k], b[k], sp[k].cut);
+      if (sp[k].cut < 8) put_y<TR>(py + row_at(r, (uint32_t)cols, (k * lanes + tl) * 8), z[k], d * rstd, rstd, w[k], b[k], sp[k].cut);
   }
 }
 
@@ -113,7 +120,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift) {
 // 74 us, now 49: 5.5 TB/s; 9000 x 16384 110 us, 5.3).
 template <class TX, class TR, int RES, int K, LoadMode MODE>
 __global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
-  __shared__ float sm[2][16];
+  __shared__ float sm[16], sm2[16][2];
   const int lanes = blockDim.x, tl = threadIdx.x, cols = (int)a.cols;
   const float inv = 1.0f / (float)cols;
   DropKey key{};
@@ -140,18 +147,21 @@ __global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
   }
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     float z[K][8];
-    const float s = join_row<TX, TR, RES, K, true, MODE>(a, key, in, sp, row, lanes, tl, z);
+    float s = join_row<TX, TR, RES, K, true, MODE>(a, key, in, sp, row, lanes, tl, z), d;
     if (row + gridDim.x < a.rows) load(row + gridDim.x);
-    const float mean = block_sum(s, sm[0]) * inv;
-    const float rstd = rsqrt_newton(block_sum(deviate<K>(z, mean, sp), sm[1]) * inv + a.eps);
+    const float mean = product(block_sum(s, sm), inv);
+    s = deviate<K>(z, mean, sp, d);
+    block_sum2(s, d, sm2);
+    d = product(d, inv);
+    const float rstd = rsqrt_newton(norm_variance(s * inv, d) + a.eps);
     if (tl == 0 && a.mean != nullptr) {
-      a.mean[row] = mean;
+      a.mean[row] = mean + d;
       a.rstd[row] = rstd;
     }
     TR* py = reinterpret_cast<TR*>(a.y) + row * a.cols;
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      if (sp[k].cut < 8) put_y<TR>(py + (k * lanes + tl) * 8, z[k], rstd, w[k], b[k], sp[k].cut);
+      if (sp[k].cut < 8) put_y<TR>(py + (k * lanes + tl) * 8, z[k], d * rstd, rstd, w[k], b[k], sp[k].cut);
   }
 }
 

@@ -1,7 +1,7 @@
 // Layer normalisation of rows beyond what a workgroup holds in registers, of any length, forward and backward: a workgroup walks a row in
 // several sweeps (the later ones find it in L2) and the gradients of weight and bias are summed by a kernel of their own that owns
 // columns.  8000 x 20000 bf16 209 us forward (3.1 TB/s of x and y), 415 us backward (2.3): three sweeps over a row instead of one.
-//   z = residual + dropout(x);  m = mean(z);  v = mean((z - m)^2);  rstd = 1 / sqrt(v + eps);  xhat = (z - m) rstd;  y = xhat w + b
+//   z = residual + dropout(x);  m = mean(z);  v = mean((z - m)^2) (norm_variance);  rstd = 1 / sqrt(v + eps);  xhat = (z - m) rstd;  y = xhat w + b
 //   g = dy w;  dz = rstd (g - mean(g) - xhat mean(g xhat));  dresidual = dz;  dx = keep ? dz scale : 0
 //   dw = sum over rows of dy xhat;  db = sum over rows of dy
 // All sums are fp32.  z is rebuilt from x, residual and the mask in the backward pass: storing it would move the same bytes (one write
@@ -42,11 +42,11 @@ __device__ __forceinline__ bool load_z(const NormArgs& a, const DropKey& key, lo
 
 template <class TX, class TR, int RES>
 __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
-  __shared__ float sm[2][16];
+  __shared__ float sm[16], sm2[16][2];
   DropKey key{};
   if (RES) key = drop_key(a.drop);
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    float s = 0.0f, z[8];
+    float s = 0.0f, d = 0.0f, z[8];
     Keep8 m;
     for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
       const int nv = (int)min(8ll, a.cols - c);
@@ -54,17 +54,22 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) s += j < nv ? z[j] : 0.0f;
     }
-    const float mean = block_sum(s, sm[0]) / (float)a.cols;
+    const float mean = block_sum(s, sm) / (float)a.cols;
     s = 0.0f;
     for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
       const int nv = (int)min(8ll, a.cols - c);
       load_z<TX, TR, RES>(a, key, row, c, nv, z, m);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s += j < nv ? (z[j] - mean) * (z[j] - mean) : 0.0f;
+      for (int j = 0; j < 8; ++j) {
+        s += j < nv ? (z[j] - mean) * (z[j] - mean) : 0.0f;
+        d += j < nv ? z[j] - mean : 0.0f;
+      }
     }
-    const float rstd = rsqrt_newton(block_sum(s, sm[1]) / (float)a.cols + a.eps);
+    block_sum2(s, d, sm2);
+    d /= (float)a.cols;                       // corrects the mean (norm.hpp)
+    const float rstd = rsqrt_newton(norm_variance(s / (float)a.cols, d) + a.eps);
     if (threadIdx.x == 0 && a.mean != nullptr) {
-      a.mean[row] = mean;
+      a.mean[row] = mean + d;
       a.rstd[row] = rstd;
     }
     for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
@@ -74,7 +79,7 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
       load_param_some<TX>(a.weight, a.p_f32, c, nv, 1.0f, w);
       load_param_some<TX>(a.bias, a.p_f32, c, nv, 0.0f, b);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) z[j] = fmaf((z[j] - mean) * rstd, w[j], b[j]);
+      for (int j = 0; j < 8; ++j) z[j] = fmaf((z[j] - mean - d) * rstd, w[j], b[j]);
       Vec8<TR> o;
       o.set(z);
       o.store(reinterpret_cast<TR*>(a.y) + row * a.cols + c, nv);

@@ -750,3 +750,74 @@ def test_block_of_the_tracker_trains():
     assert off(y, y64) < 1000 * E32 and off(y2, y64) < 1000 * E32
     for k in t:
         assert off(a[k].grad, b[k].grad) < 1000 * E32, (k, off(a[k].grad, b[k].grad))
+
+
+# ---------------------------------------------------------------------------------------------- rows far from zero
+
+def offset_bounds(o, eps, dtype):
+    """Tolerances where the mean is far larger than the spread (types: all `dtype`, parameters fp32, z exact in fp32).  depth as above.
+    The first mean is off by delta <= e (depth + 2) mean|z|; the deviations from it are off by e of themselves; their mean, by which they are
+    corrected, by e (depth + 3) mean|z - first| <= e (depth + 3) (delta + MAD); the variance by e (depth + 8) (var + delta^2).  So
+      E = e rstd ((depth + 8) (delta + MAD) + 2 |z - mean|) + e (depth + 16) |xhat| (1 + delta^2 / (var + eps))
+    of which only e^2 mean|z| grows with the offset.  The backward pass takes z from the stored mean, an fp32 number:
+      Eb = E + e |mean| rstd,  and from there the module's formulas."""
+    D = o["z"].shape[-1]
+    depth = 8 * math.ceil(D / 2048) + 32
+    mean = lambda t: t.mean(-1, keepdim=True)        # noqa: E731
+    dev = (o["z"] - o["mean"]).abs()
+    delta = E32 * (depth + 2) * mean(o["z"].abs())
+    E = E32 * o["rstd"] * ((depth + 8) * (delta + mean(dev)) + 2 * dev) + E32 * (depth + 16) * o["xhat"].abs() * (1 + (delta * o["rstd"]) ** 2)
+    t = {"y": u(dtype) * o["y"].abs() + o["w"].abs() * E + 4 * E32 * ((o["xhat"] * o["w"]).abs() + o["b"].abs()) + tiny(dtype),
+         "mean": E32 * o["mean"].abs() + E32 * (depth + 3) * (delta + mean(dev)),
+         "rstd": E32 * (depth + 16) * o["rstd"] * (1 + (delta * o["rstd"]) ** 2)}
+    Eb = E + E32 * o["mean"].abs() * o["rstd"]
+    g, xh, dz = o["g"].abs(), o["xhat"].abs() + Eb, o["dresidual"].abs()
+    raw = o["rstd"] * (4 * E32 * g + E32 * (depth + 4) * mean(g) + xh * (E32 * (depth + 4) * mean(g * xh) + mean(g * Eb)) + Eb * o["c2"].abs()) \
+        + E32 * (depth + 16) * (1 + (delta * o["rstd"]) ** 2) * dz
+    rows = o["z"].numel() // D
+    n = min(rows, rows / 64 + 64) + 32
+    flat = lambda v: v.reshape(-1, D).sum(0)         # noqa: E731
+    t["dx"] = t["dresidual"] = u(dtype) * dz + raw + tiny(dtype)
+    t["dweight"] = u(F32) * o["dweight"].abs() + flat(o["dy"].abs() * Eb) + E32 * n * flat(o["dy"].abs() * xh)
+    return t
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("cols", [5, 257, 768, 1000, 1537, 5000, 17000])
+def test_norm_rows_far_from_zero(dtype, cols):
+    """Constant rows, rows that are constant but for one element, and small spreads on large offsets: what is left is the spread's, whatever the
+    offset is; layer_norm and the join (whose sum is exact here: the residual holds the other half)."""
+    offsets = [1000.0, 1000.1, 65504.0, 30000.3, -12345.6, 0.1, 3.0]
+    rows = torch.tensor(offsets).repeat_interleave(3)[:, None].repeat(1, cols)
+    step = torch.finfo(dtype).eps * torch.tensor(offsets).abs()
+    for i in range(len(offsets)):
+        rows[3 * i + 1, cols // 3] -= 2 * step[i]                                     # one element two steps lower
+        rows[3 * i + 2] -= 4 * step[i] * torch.randint(0, 3, (cols,), generator=torch.Generator().manual_seed(i)) * torch.sign(rows[3 * i + 2])
+    g = torch.Generator().manual_seed(cols)
+    w, b = 1 + 0.2 * torch.randn(cols, generator=g), 0.2 * torch.randn(cols, generator=g)
+    dy = torch.randn(*rows.shape, generator=g).to(dtype)
+    x = rows.to(dtype)
+    for joined in (False, True):
+        half = (x.float() / 2).to(dtype) if joined else x                              # exact: a power of two
+        r = half if joined else None
+        want = ref.norm(half, w, b, 1e-5, r, None, dy)
+        tol = offset_bounds(want, 1e-5, dtype)
+        dev = lambda t: None if t is None else t.cuda()                                # noqa: E731
+        y, mean, rstd = hip.norm_forward(dev(half), dev(w), dev(b), 1e-5, dev(r), want_stats=True)
+        within(y, want["y"], tol["y"], "y")
+        within(mean[:, None], want["mean"], tol["mean"], "mean")
+        within(rstd[:, None], want["rstd"], tol["rstd"], "rstd")
+        dx, dres, dw, _ = hip.norm_backward(dev(dy), dev(half), mean, rstd, dev(w), dev(b), 1e-5, dev(r))
+        within(dx, want["dx"], tol["dx"], "dx")
+        if joined:
+            within(dres, want["dresidual"], tol["dresidual"], "dresidual")
+        within(dw, want["dweight"], tol["dweight"], "dweight")
+
+
+@gpu
+def test_norm_constant_rows_at_small_eps():
+    """No eps makes something of the rounding of a constant row: below 2^-18 of the squares that the first mean leaves, a variance is noise."""
+    x = torch.tensor([1000.1, -30000.3, 0.1])[:, None].repeat(1, 1000).cuda()
+    for eps in (1e-5, 1e-12, 1e-30, 1.2e-38):
+        assert float(layer_norm(x, eps=eps).abs().max()) < 2 ** 9 * E32 * 64, eps
