@@ -16,7 +16,8 @@ int make_drop(double p, uint64_t seed, const void* seed_ptr, uint64_t offset, Dr
   return 0;
 }
 
-// A thread takes one chunk of eight elements, which is one block of the generator, and ends: bound by HBM (67108864 bf16 46 us, 5.8 TB/s;
+// A thread takes one chunk of eight elements, which is one block of the generator, and ends (beyond 2^35 elements it strides, since a launch
+// holds no more threads): bound by HBM (67108864 bf16 46 us, 5.8 TB/s;
 // 150994944 bf16 99 us, 6.1; fp32 207 us, 5.8: its lanes lie 32 bytes apart).  A grid that strides over the chunks
 // instead reached 4.4 - 5.0 TB/s; the ten rounds are hidden behind the memory (0, 7 or 10 of them: 345, 347, 342 us a GiB).
 template <class T>
@@ -45,7 +46,7 @@ int dropout(const void* x, void* y, long long n, int type, const DropArgs& d, hi
   if (n == 0) return 0;
   ProfScope prof("dropout", stream, 3.0 * n, 2.0 * n * elem_size(type));
   const long long chunks = (n + 7) >> 3, want = (chunks + 255) / 256;
-  const unsigned grid = (unsigned)(want < (1ll << 30) ? want : (1ll << 30));
+  const unsigned grid = grid_of(want, 256);
   switch (type) {
     case kF32: dropout_kernel<float><<<grid, 256, 0, stream>>>((const float*)x, (float*)y, n, d); break;
     case kF16: dropout_kernel<_Float16><<<grid, 256, 0, stream>>>((const _Float16*)x, (_Float16*)y, n, d); break;

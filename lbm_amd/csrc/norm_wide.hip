@@ -171,13 +171,13 @@ int norm_wide_parts(long long rows, long long cols) {
 }
 
 template <class TX, class TR, int RES> static int wide_forward(const NormArgs& a, hipStream_t s) {
-  const unsigned grid = (unsigned)(a.rows < (1ll << 30) ? a.rows : (1ll << 30));
+  const unsigned grid = grid_of(a.rows, 256);
   norm_wide_fwd_kernel<TX, TR, RES><<<grid, 256, 0, s>>>(a);
   return check_launch("norm_forward");
 }
 template <class TX, class TR, int RES> static int wide_backward(const NormArgs& a, hipStream_t s) {
   if (a.rows > 0 && (a.dx != nullptr || a.dresidual != nullptr)) {
-    const unsigned grid = (unsigned)(a.rows < (1ll << 30) ? a.rows : (1ll << 30));
+    const unsigned grid = grid_of(a.rows, 256);
     norm_wide_dx_kernel<TX, TR, RES><<<grid, 256, 0, s>>>(a);
     if (check_launch("norm_backward")) return -1;
   }

@@ -2,6 +2,7 @@
 // counter-based generator and layer normalisation with its gradients.  Shared declarations and device helpers.
 #pragma once
 #include "common.hpp"
+#include "launch.hpp"
 
 namespace lbm {
 

@@ -821,3 +821,38 @@ def test_norm_constant_rows_at_small_eps():
     x = torch.tensor([1000.1, -30000.3, 0.1])[:, None].repeat(1, 1000).cuda()
     for eps in (1e-5, 1e-12, 1e-30, 1.2e-38):
         assert float(layer_norm(x, eps=eps).abs().max()) < 2 ** 9 * E32 * 64, eps
+
+
+# ---------------------------------------------------------------------------------------------- sizes beyond one launch
+
+def test_grids_stay_below_what_a_launch_holds(tmp_path):
+    """launch.hpp, compiled by itself: HIP takes fewer than 2^32 threads along a dimension."""
+    import os
+    import subprocess
+    src, lib = tmp_path / "launch.cpp", tmp_path / "launch.so"
+    src.write_text('#include "launch.hpp"\nextern "C" unsigned grid(long long want, int threads) { return lbm::grid_of(want, threads); }\n')
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "lbm_amd", "csrc")
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-I", csrc, str(src), "-o", str(lib)], check=True)
+    grid = C.CDLL(str(lib)).grid
+    grid.argtypes, grid.restype = [C.c_longlong, C.c_int], C.c_uint
+    for threads in (64, 192, 256, 1024):
+        for want in (1, 255, 1 << 22, (1 << 24) - 1, 1 << 24, 1 << 26, 1 << 30, 1 << 40):
+            g = grid(want, threads)
+            assert 1 <= g <= want and g * threads < 1 << 32
+            assert g == want or (g + 1) * threads >= 1 << 32
+
+
+@gpu
+def test_dropout_beyond_one_launch():
+    """2^35 elements are 2^32 threads' work: the last chunks are a thread's second."""
+    n, p, seed, offset = (1 << 35) + 4099, 0.25, 42, 7
+    lib = hip.load()
+    torch.cuda.empty_cache()
+    x = torch.ones(n, device="cuda", dtype=F16)
+    assert lib.lbm_hip_dropout(x.data_ptr(), x.data_ptr(), n, 1, p, seed, None, offset, torch.cuda.current_stream().cuda_stream) == 0, lib.lbm_hip_last_error()
+    for first in (0, (1 << 32) - 1000, (1 << 35) - 3048, n - 2000):
+        got = x[first:first + 2000].float().cpu()
+        want = ref.keep((2000,), p, seed, offset, first=first)
+        assert torch.equal(got != 0, want) and torch.equal(got[want], torch.full((int(want.sum()),), ref.scale(p)).half().float())
+    del x
+    torch.cuda.empty_cache()
