@@ -1,6 +1,8 @@
 // Layer normalisation with the row in registers: y = (z - mean) rstd w + b, z = x or residual + dropout(x).
 // One sweep over memory: a team of threads (norm.hpp) loads its row, sums it, sums the deviations from that mean and their squares (the
 // two-pass form; the deviations' own mean corrects the first one, norm.hpp) and writes y.  Bound by HBM: x (and residual) in, y out.
+#include <algorithm>
+
 #include "norm.hpp"
 
 namespace lbm {
@@ -66,7 +68,7 @@ template <class TR> __device__ __forceinline__ void put_y(TR* y, float (&z)[8], 
 // keeps the whole chip on neighbouring pages.  589824 x 256 bf16 107 us (5.6 TB/s), the join 158 us (5.7); 583657 x 257 134 us (4.5: the 33rd
 // chunk of a row has a stripe of its own).  Beside HBM the vector instructions are next: half of the issue slots at 256 columns.
 template <class TX, class TR, int RES, int K, int U, LoadMode MODE>
-__global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift) {
+__global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift, long long first) {
   const int lanes = 1 << shift, tl = threadIdx.x & (lanes - 1), team = threadIdx.x >> shift, teams = 256 >> shift, cols = (int)a.cols;
   const float inv = 1.0f / (float)cols;
   DropKey key{};
@@ -74,7 +76,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift) {
   Span sp[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) sp[k] = Span::of<MODE>((k * lanes + tl) * 8, cols, k == K - 1);
-  const long long base = (long long)blockIdx.x * (teams * U);
+  const long long base = first + (long long)blockIdx.x * (teams * U);
   const int last = (int)min((long long)(teams * U), a.rows - base) - 1;          // of this workgroup's rows
   const TX* px = reinterpret_cast<const TX*>(a.x) + base * a.ld_x;
   const TR* pr = reinterpret_cast<const TR*>(a.residual) + base * a.ld_r;
@@ -172,10 +174,13 @@ constexpr long long kManyGroups = 2048;
 // (97656 x 1536: 156 us, 179 in a workgroup).
 template <int RES> constexpr int wave_chunks() { return RES ? 192 : 256; }
 template <class TX, class TR, int RES, int K, int U, LoadMode MODE> static int wave_forward(const NormArgs& a, const NormShape& sh, hipStream_t s) {
-  const long long per = (long long)sh.teams() * U, grid = (a.rows + per - 1) / per;
-  LBM_REQUIRE(grid < (1ll << 31), "norm_forward: %lld rows are more than a grid holds", a.rows);
-  norm_fwd_kernel<TX, TR, RES, K, U, MODE><<<(unsigned)grid, 256, 0, s>>>(a, sh.shift);
-  return check_launch("norm_forward");
+  const long long per = (long long)sh.teams() * U, most = grid_most(256) * per;
+  for (long long first = 0; first < a.rows; first += most) {       // more than one launch: rows of fewer than eight columns, 2^32 and more of them
+    const long long rows = std::min(most, a.rows - first);
+    norm_fwd_kernel<TX, TR, RES, K, U, MODE><<<(unsigned)((rows + per - 1) / per), 256, 0, s>>>(a, sh.shift, first);
+    if (check_launch("norm_forward")) return -1;
+  }
+  return 0;
 }
 template <class TX, class TR, int RES, LoadMode MODE> static int forward_rows(const NormArgs& a, hipStream_t s) {
   const NormShape sh = norm_shape(a.cols, wave_chunks<RES>());

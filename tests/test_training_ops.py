@@ -856,3 +856,29 @@ def test_dropout_beyond_one_launch():
         assert torch.equal(got != 0, want) and torch.equal(got[want], torch.full((int(want.sum()),), ref.scale(p)).half().float())
     del x
     torch.cuda.empty_cache()
+
+
+@gpu
+def test_norm_forward_beyond_one_launch():
+    """2^32 rows of two columns and some: the last ones belong to a second launch.  With statistics of every row: 34 GB."""
+    rows, cols, p, seed, offset = (1 << 32) + 1003, 2, 0.3, 11, 4
+    torch.cuda.empty_cache()
+    g = torch.Generator("cuda").manual_seed(10)
+    x = torch.empty(rows, cols, device="cuda", dtype=F16)
+    x.view(-1)[:1 << 20].normal_(generator=g)
+    n = 1 << 20
+    while n < x.numel():                                                              # a pattern of 2^20 numbers over all of it
+        k = min(n, x.numel() - n)
+        x.view(-1)[n:n + k] = x.view(-1)[:k]
+        n += k
+    w, b = torch.tensor([1.25, -0.5], device="cuda"), torch.tensor([0.1, 0.2], device="cuda")
+    y, mean, rstd = hip.norm_forward(x, w, b, 1e-5, x, p, seed, offset, want_stats=True)
+    edge = ((1 << 24) - 1) * 256
+    for first in (0, (1 << 31) - 3, edge - 500, rows - 1000):
+        part = slice(first, first + 1000)
+        factor = ref.keep((1000, cols), p, seed, offset, first=first * cols).double() * ref.scale(p)
+        want = ref.norm(x[part], w, b, 1e-5, x[part], factor)
+        within(y[part], want["y"], bounds(want, 1e-5, F16, F16, F32, ref.scale(p))["y"], "y")
+        within(mean[part][:, None], want["mean"], 4 * E32 * (want["z"].abs() + want["xs"].abs()).mean(-1, keepdim=True) + 2.0 ** -140, "mean")
+    del x, y, mean, rstd
+    torch.cuda.empty_cache()
