@@ -263,26 +263,29 @@ template <class T>
 __global__ __launch_bounds__(1024) void norm_finish_kernel(const float* part, int parts, long long cols, T* dweight, T* dbias) {
   __shared__ float sm[32][33];
   const int tc = threadIdx.x & 31, tg = threadIdx.x >> 5;
-  const long long c = (long long)blockIdx.x * 32 + tc;              // over 2 cols: dweight, then dbias
-  float s = 0.0f;
-  if (c < 2 * cols) {
-    const float* p = part + c;
+  for (long long c0 = (long long)blockIdx.x * 32; c0 < 2 * cols; c0 += (long long)gridDim.x * 32) {      // over 2 cols: dweight, then dbias
+    const long long c = c0 + tc;
+    float s = 0.0f;
+    if (c < 2 * cols) {
+      const float* p = part + c;
 #pragma unroll 8
-    for (int g = tg; g < parts; g += 32) s += p[(long long)g * 2 * cols];
-  }
-  sm[tg][tc] = s;
-  __syncthreads();
-  if (tg < 1 && c < 2 * cols) {
-    s = 0.0f;
+      for (int g = tg; g < parts; g += 32) s += p[(long long)g * 2 * cols];
+    }
+    sm[tg][tc] = s;
+    __syncthreads();
+    if (tg < 1 && c < 2 * cols) {
+      s = 0.0f;
 #pragma unroll
-    for (int g = 0; g < 32; ++g) s += sm[g][tc];
-    T* o = c < cols ? dweight : dbias;
-    if (o != nullptr) o[c < cols ? c : c - cols] = (T)s;
+      for (int g = 0; g < 32; ++g) s += sm[g][tc];
+      T* o = c < cols ? dweight : dbias;
+      if (o != nullptr) o[c < cols ? c : c - cols] = (T)s;
+    }
+    __syncthreads();
   }
 }
 
 int norm_finish(const NormArgs& a, int parts, hipStream_t s) {
-  const unsigned grid = (unsigned)((2 * a.cols + 31) / 32);
+  const unsigned grid = grid_of((2 * a.cols + 31) / 32, 1024);      // beyond 2^26 columns it strides
   if (a.p_f32) norm_finish_kernel<float><<<grid, 1024, 0, s>>>(a.workspace, parts, a.cols, (float*)a.dweight, (float*)a.dbias);
   else if (a.x_type == kF16) norm_finish_kernel<_Float16><<<grid, 1024, 0, s>>>(a.workspace, parts, a.cols, (_Float16*)a.dweight, (_Float16*)a.dbias);
   else norm_finish_kernel<__bf16><<<grid, 1024, 0, s>>>(a.workspace, parts, a.cols, (__bf16*)a.dweight, (__bf16*)a.dbias);

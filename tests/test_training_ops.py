@@ -882,3 +882,31 @@ def test_norm_forward_beyond_one_launch():
         within(mean[part][:, None], want["mean"], 4 * E32 * (want["z"].abs() + want["xs"].abs()).mean(-1, keepdim=True) + 2.0 ** -140, "mean")
     del x, y, mean, rstd
     torch.cuda.empty_cache()
+
+
+@gpu
+@pytest.mark.parametrize("bias", [True, False])
+def test_norm_columns_beyond_one_launch(bias):
+    """2^26 columns and some: their sums are 2^32 threads' work.  dy is zero but for a few columns, so that the oracle's sums are short."""
+    rows, cols = 2, (1 << 26) + 4001
+    g = torch.Generator("cuda").manual_seed(12)
+    x = torch.empty(rows, cols, device="cuda", dtype=F16).normal_(generator=g)
+    w = torch.ones(cols, device="cuda", dtype=F16)
+    dy = torch.zeros(rows, cols, device="cuda", dtype=F16)
+    at = torch.tensor([0, 5, (1 << 25) + 3, (1 << 26) - 1, 1 << 26, cols - 1], device="cuda")
+    dy[:, at] = torch.randn(rows, len(at), device="cuda", generator=g).half()
+    # statistics that are given, not computed: what is checked is the sums over rows
+    mean, rstd = torch.tensor([0.25, -0.5], device="cuda"), torch.tensor([1.5, 0.75], device="cuda")
+    _, _, dw, db = hip.norm_backward(dy, x, mean, rstd, w, w if bias else None, want=(False, False, True, bias))
+    term = dy[:, at].double() * (x[:, at].double() - mean[:, None].double()) * rstd[:, None].double()
+    want = torch.zeros(cols, device="cuda", dtype=torch.float64)
+    want[at] = term.sum(0)
+    tol = torch.zeros_like(want)
+    tol[at] = u(F16) * want[at].abs() + 8 * E32 * term.abs().sum(0) + tiny(F16)
+    within(dw, want.cpu(), tol.cpu(), "dweight")
+    if bias:
+        want[at] = dy[:, at].double().sum(0)
+        tol[at] = u(F16) * want[at].abs() + 8 * E32 * dy[:, at].double().abs().sum(0) + tiny(F16)
+        within(db, want.cpu(), tol.cpu(), "dbias")
+    else:
+        assert db is None
