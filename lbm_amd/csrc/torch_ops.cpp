@@ -328,6 +328,8 @@ Tensor dropout(const Tensor& x, const Drop& drop) {
 }
 
 Tensor norm(const char* what, const Tensor& x, const Tensor& residual, const Tensor& weight, const Tensor& bias, double eps, const Drop& drop) {
+  for (const Tensor* t : {&x, &residual, &weight, &bias})
+    if (t->defined()) elem_type(*t, what);       // before refuse(), which asks the GPU
   const bool grad = c10::GradMode::is_enabled() && (wants_grad(x) || wants_grad(residual) || wants_grad(weight) || wants_grad(bias));
   refuse(what, {&x, &residual, &weight, &bias}, grad);
   std::tuple<Tensor, Tensor> r;

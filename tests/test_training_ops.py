@@ -910,3 +910,14 @@ def test_norm_columns_beyond_one_launch(bias):
         within(db, want.cpu(), tol.cpu(), "dbias")
     else:
         assert db is None
+
+
+# ---------------------------------------------------------------------------------------------- the host path
+
+def test_cpu_tensors_that_want_gradients_are_refused():
+    """The documented error, also where the machine has no GPU to be asked."""
+    x, w = torch.zeros(2, 8, requires_grad=True), torch.ones(8, requires_grad=True)
+    for call in (lambda: layer_norm(x), lambda: layer_norm(x, w, w), lambda: layer_norm(x.detach(), w), lambda: dropout(x, 0.5, 1),
+                 lambda: dropout_add_layer_norm(x, x, w), lambda: dropout_add_layer_norm(x.detach(), x)):
+        with pytest.raises(hip.HipError, match="GPU"):
+            call()
