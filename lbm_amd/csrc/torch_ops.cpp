@@ -291,12 +291,15 @@ bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 // What a graph of these operators would get wrong without an error: forward-mode derivatives, which they do not carry on; and a step
 // captured while an eager graph on the default stream still holds the leaves -- the backward pass would make that stream wait
-// inside the capture, which the default stream cannot.
+// inside the capture, which the default stream cannot.  `inputs`: x first, whose device's stream the operator runs on.
 void refuse(const char* what, std::initializer_list<const Tensor*> inputs, bool grad) {
   for (const Tensor* t : inputs)
     if (t->defined() && t->_fw_grad(0).defined()) fail(std::string(what) + ": forward-mode derivatives are not supported");
   // (the default stream cannot capture, and asking it while another stream does is an error)
-  if (!grad || c10::hip::getCurrentHIPStream().id() == 0 || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const c10::Device device = (*inputs.begin())->device();
+  if (!grad || c10::hip::getCurrentHIPStream(device.index()).id() == 0) return;
+  const c10::DeviceGuard guard(device);
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   for (const Tensor* t : inputs) {
     if (!wants_grad(*t) || !t->is_leaf()) continue;
     const auto leaf = torch::autograd::impl::try_get_grad_accumulator(*t);

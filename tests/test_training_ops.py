@@ -921,3 +921,22 @@ def test_cpu_tensors_that_want_gradients_are_refused():
                  lambda: dropout_add_layer_norm(x, x, w), lambda: dropout_add_layer_norm(x.detach(), x)):
         with pytest.raises(hip.HipError, match="GPU"):
             call()
+
+
+@gpu
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_capture_on_a_device_that_is_not_the_current_one():
+    """The refusal beside a living eager graph asks the stream of x's device, whichever device is current."""
+    w = torch.ones(32, device="cuda:1").requires_grad_()
+    x = torch.randn(4, 32, device="cuda:1")
+    alive = layer_norm(x, w)
+    torch.cuda.synchronize(1)
+    side = torch.cuda.Stream(device="cuda:1")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.device(1), torch.cuda.stream(side):
+        graph.capture_begin()
+        out = x + 1
+        with torch.cuda.device(0), pytest.raises(hip.HipError, match="eager graph"):
+            layer_norm(x, w)
+        graph.capture_end()
+    del alive, out
