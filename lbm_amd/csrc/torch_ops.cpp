@@ -91,6 +91,10 @@ struct Drop {
   Tensor seed_dev;                               // defined: read by the kernel in place of seed
   const void* address() const { return seed_dev.defined() ? seed_dev.const_data_ptr() : nullptr; }
 };
+void check_seed(const char* what, const Tensor& seed, c10::Device device) {
+  if (seed.scalar_type() != at::kLong || seed.numel() != 1 || seed.device() != device)
+    fail(std::string(what) + ": a seed tensor holds one int64 on the operands' device, got " + text(seed));
+}
 Drop make_drop(const char* what, double p, uint64_t seed, const std::optional<Tensor>& seed_dev, uint64_t offset, const Tensor& x) {
   Drop d;
   if (!(p >= 0.0 && p <= 1.0)) fail(std::string(what) + ": p = " + std::to_string(p) + " is not a probability");
@@ -99,8 +103,7 @@ Drop make_drop(const char* what, double p, uint64_t seed, const std::optional<Te
   d.offset = offset;
   if (seed_dev.has_value() && seed_dev->defined()) {
     d.seed_dev = *seed_dev;
-    if (d.seed_dev.scalar_type() != at::kLong || d.seed_dev.numel() != 1 || d.seed_dev.device() != x.device())
-      fail(std::string(what) + ": a seed tensor holds one int64 on the operands' device, got " + text(d.seed_dev));
+    check_seed(what, d.seed_dev, x.device());
   }
   return d;
 }
@@ -248,14 +251,20 @@ struct NormBackward : public Node {
       fail("the gradients of layer_norm and dropout_add_layer_norm are not differentiable (create_graph=True)");
     if (!grads[0].defined()) return variable_list(4);
     const Tensor tx = x.unpack(), tr = residual.unpack(), tw = weight.unpack(), ts = seed.unpack();
+    // hooks on saved tensors may return anything; the kernels take every size and type from x and residual, and the statistics from the forward pass
+    const Tensor& dy = grads[0];
+    const Tensor& like = tr.defined() ? tr : tx;
+    if (dy.sizes() != tx.sizes() || dy.scalar_type() != like.scalar_type() || dy.device() != tx.device() || (tw.defined() && tw.scalar_type() != p_scalar))
+      fail("norm_backward: a saved tensor came back with another size, type or device: x " + text(tx) + ", the forward pass's result was like " + text(dy));
     Operands o = operands("norm_backward", tx, tr, tw, Tensor());
     o.bias = bias;
     o.p_type = p_type;
     o.p_scalar = p_scalar;
     Drop d = drop;
     d.seed_dev = ts;
+    if (ts.defined()) check_seed("norm_backward", ts, dy.device());
     const float* mean = (const float*)stats.const_data_ptr();
-    return run_backward(o, eps, d, grads[0], mean, mean + o.rows, task_should_compute_output(0), task_should_compute_output(1),
+    return run_backward(o, eps, d, dy, mean, mean + o.rows, task_should_compute_output(0), task_should_compute_output(1),
                         task_should_compute_output(2), task_should_compute_output(3));
   }
   void release_variables() override {
@@ -278,6 +287,7 @@ struct DropoutBackward : public Node {
     if (!grads[0].defined()) return variable_list(1);
     Drop d = drop;
     d.seed_dev = seed.unpack();
+    if (d.seed_dev.defined()) check_seed("dropout_backward", d.seed_dev, grads[0].device());
     return {dropout(grads[0], d)};
   }
   void release_variables() override {

@@ -940,3 +940,33 @@ def test_capture_on_a_device_that_is_not_the_current_one():
             layer_norm(x, w)
         graph.capture_end()
     del alive, out
+
+
+@gpu
+@pytest.mark.parametrize("joined", [False, True])
+def test_saved_tensors_that_come_back_different_are_refused(joined):
+    """Hooks that change size, type or device: the backward pass would read dy in another type or beyond its end."""
+    def run(unpack):
+        x, r, w = torch.randn(6, 40, device="cuda"), torch.randn(6, 40, device="cuda"), torch.ones(40, device="cuda")
+        x.requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y = dropout_add_layer_norm(x, r, w, p=0.2, seed=1) if joined else layer_norm(x, w)
+        return torch.autograd.grad(y, x, torch.ones_like(y))
+
+    run(lambda t: t.clone())
+    changes = [lambda t: t.half(), lambda t: torch.cat([t, t]), lambda t: t.cpu(), lambda t: t[..., :20], lambda t: t[:3], lambda t: t.half() if t.dim() == 1 else t,
+               lambda t: t[:20] if t.dim() == 1 else t, lambda t: t.double()]
+    for k, change in enumerate(changes):
+        with pytest.raises(hip.HipError):
+            run(change)
+
+
+@gpu
+def test_saved_seeds_that_come_back_different_are_refused():
+    x, seed = torch.randn(6, 40, device="cuda").requires_grad_(), torch.tensor([3], device="cuda")
+    for call in (lambda: dropout(x, 0.5, seed), lambda: dropout_add_layer_norm(x, x, p=0.5, seed=seed)):
+        for change in (lambda t: t.cpu(), lambda t: t.int(), lambda t: t.expand(2)):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: change(t) if t.dtype == torch.int64 else t):
+                y = call()
+            with pytest.raises(hip.HipError, match="seed"):
+                torch.autograd.grad(y, x, torch.ones_like(y))
