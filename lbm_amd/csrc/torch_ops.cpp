@@ -53,6 +53,7 @@ std::string text(const Tensor& t) {
 int elem_type(const Tensor& t, const char* what) {
   TORCH_CHECK(api.forward != nullptr, "lbm_amd._torch_ops is used through lbm_amd.hip.ops()");
   if (!t.is_cuda()) fail(std::string(what) + ": expected a GPU tensor, got " + text(t));
+  if (!t.has_storage()) fail(std::string(what) + ": expected a plain dense tensor (no torch.func transform, no sparse layout), got " + text(t));
   switch (t.scalar_type()) {
     case at::kFloat: return LBM_TYPE_F32;
     case at::kHalf: return LBM_TYPE_F16;
@@ -92,7 +93,7 @@ struct Drop {
   const void* address() const { return seed_dev.defined() ? seed_dev.const_data_ptr() : nullptr; }
 };
 void check_seed(const char* what, const Tensor& seed, c10::Device device) {
-  if (seed.scalar_type() != at::kLong || seed.numel() != 1 || seed.device() != device)
+  if (!seed.has_storage() || seed.scalar_type() != at::kLong || seed.numel() != 1 || seed.device() != device)
     fail(std::string(what) + ": a seed tensor holds one int64 on the operands' device, got " + text(seed));
 }
 Drop make_drop(const char* what, double p, uint64_t seed, const std::optional<Tensor>& seed_dev, uint64_t offset, const Tensor& x) {
@@ -253,6 +254,7 @@ struct NormBackward : public Node {
     const Tensor tx = x.unpack(), tr = residual.unpack(), tw = weight.unpack(), ts = seed.unpack();
     // hooks on saved tensors may return anything; the kernels take every size and type from x and residual, and the statistics from the forward pass
     const Tensor& dy = grads[0];
+    elem_type(dy, "norm_backward");
     const Tensor& like = tr.defined() ? tr : tx;
     if (dy.sizes() != tx.sizes() || dy.scalar_type() != like.scalar_type() || dy.device() != tx.device() || (tw.defined() && tw.scalar_type() != p_scalar))
       fail("norm_backward: a saved tensor came back with another size, type or device: x " + text(tx) + ", the forward pass's result was like " + text(dy));

@@ -970,3 +970,23 @@ def test_saved_seeds_that_come_back_different_are_refused():
                 y = call()
             with pytest.raises(hip.HipError, match="seed"):
                 torch.autograd.grad(y, x, torch.ones_like(y))
+
+
+@gpu
+def test_function_transforms_and_sparse_tensors_are_refused():
+    """torch.func's wrappers and sparse tensors have no memory to hand to a kernel: an error that says so, for operands and gradients."""
+    x, w = torch.randn(3, 4, 16, device="cuda"), torch.ones(16, device="cuda")
+    f = torch.func
+    for call in (lambda: f.vmap(layer_norm)(x), lambda: f.vmap(lambda v: dropout(v, 0.5, 1))(x), lambda: f.vmap(lambda v: dropout_add_layer_norm(v, v))(x),
+                 lambda: f.grad(lambda v: layer_norm(v).sum())(x), lambda: f.grad(lambda v: dropout(v, 0.5, 1).sum())(x),
+                 lambda: f.grad(lambda v: layer_norm(x, v).sum())(w), lambda: f.vmap(lambda v: layer_norm(x, v))(torch.stack([w, w])),
+                 lambda: f.vmap(lambda v: hip.norm_forward(v, None, None))(x), lambda: dropout(x.to_sparse(), 0.5, 1), lambda: layer_norm(x[0].to_sparse())):
+        with pytest.raises(hip.HipError, match="plain dense tensor"):
+            call()
+    for op in (lambda t: layer_norm(t), lambda t: dropout(t, 0.5, 1)):
+        leaf = x[0].clone().requires_grad_()
+        y = op(leaf)
+        with pytest.raises(hip.HipError, match="plain dense tensor"):
+            torch.nn.functional.embedding(torch.tensor([0, 2], device="cuda"), y, sparse=True).sum().backward()
+    with pytest.raises(hip.HipError, match="seed"):
+        f.vmap(lambda s: dropout(x, 0.5, s))(torch.arange(3, device="cuda"))
