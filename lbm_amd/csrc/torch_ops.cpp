@@ -62,8 +62,12 @@ int elem_type(const Tensor& t, const char* what) {
   }
 }
 
+// a view that torch negates when it reads it (the imaginary part of a conjugate): a copy
+Tensor as_stored(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // Rows of the last dimension at one stride are used where they lie, any other layout is copied; ld: elements between rows
-Tensor as_rows(const Tensor& t, int64_t& ld) {
+Tensor as_rows(const Tensor& given, int64_t& ld) {
+  const Tensor t = as_stored(given);
   const int64_t n = t.size(-1);
   ld = n;
   if (t.is_contiguous()) return t;
@@ -121,7 +125,7 @@ struct Operands {
 Tensor param(const char* what, const Tensor& p, const Operands& o) {
   if (p.dim() != 1 || p.size(0) != o.cols || p.device() != o.x.device())
     fail(std::string(what) + ": weight / bias are (" + std::to_string(o.cols) + ") on " + o.x.device().str() + ", got " + text(p));
-  return p.is_contiguous() ? p : p.contiguous();
+  return as_stored(p).contiguous();
 }
 Operands operands(const char* what, const Tensor& x, const Tensor& residual, const Tensor& weight, const Tensor& bias) {
   Operands o;
@@ -228,7 +232,7 @@ variable_list run_backward(const Operands& o, double eps, const Drop& drop, cons
 Tensor run_dropout(const Tensor& x, const Drop& drop) {
   const int type = elem_type(x, "dropout");
   const c10::DeviceGuard guard(x.device());
-  const Tensor dense = x.contiguous();
+  const Tensor dense = as_stored(x).contiguous();
   Tensor y = at::empty(x.sizes(), x.options());
   checked(api.dropout(address(dense), y.mutable_data_ptr(), x.numel(), type, drop.p, drop.seed, drop.address(), drop.offset, stream_of(x)), "lbm_hip_dropout");
   return y;

@@ -990,3 +990,23 @@ def test_function_transforms_and_sparse_tensors_are_refused():
             torch.nn.functional.embedding(torch.tensor([0, 2], device="cuda"), y, sparse=True).sum().backward()
     with pytest.raises(hip.HipError, match="seed"):
         f.vmap(lambda s: dropout(x, 0.5, s))(torch.arange(3, device="cuda"))
+
+
+@gpu
+def test_negative_views():
+    """The imaginary part of a conjugate is a view that torch negates when it is read."""
+    g = torch.Generator("cuda").manual_seed(31)
+    bits = lambda *shape: torch.randn(*shape, dtype=torch.complex64, device="cuda", generator=g).conj().imag.as_strided(shape, torch.empty(shape).stride())     # noqa: E731
+    x, r, w, b, dy = bits(6, 40), bits(6, 40), bits(40), bits(40), bits(6, 40)
+    assert all(t.is_neg() and t.is_contiguous() for t in (x, r, w, b, dy))
+    plain = [t.resolve_neg() for t in (x, r, w, b)]
+    assert torch.equal(dropout(x, 0.4, 3, 1), dropout(plain[0], 0.4, 3, 1))
+    assert torch.equal(layer_norm(x[0:1, 4:], w[4:], b[4:]), layer_norm(plain[0][0:1, 4:], plain[2][4:], plain[3][4:]))
+    results = []
+    for t, d in (((x, r, w, b), dy), (plain, dy.resolve_neg())):
+        leaves = [v.detach().requires_grad_() for v in t]
+        y = dropout_add_layer_norm(*leaves, p=0.3, seed=2)
+        results.append([y.detach(), *torch.autograd.grad(y, leaves, d)])
+    assert all(torch.equal(p, q) for p, q in zip(*results))
+    leaf = plain[0].detach().requires_grad_()
+    assert torch.equal(torch.autograd.grad(dropout(leaf, 0.4, 3), leaf, dy)[0], dropout(dy.resolve_neg(), 0.4, 3))
