@@ -4,7 +4,7 @@
 //   z = residual + dropout(x);  m = mean(z);  v = mean((z - m)^2) (norm_variance);  rstd = 1 / sqrt(v + eps);  xhat = (z - m) rstd;  y = xhat w + b
 //   g = dy w;  dz = rstd (g - mean(g) - xhat mean(g xhat));  dresidual = dz;  dx = keep ? dz scale : 0
 //   dw = sum over rows of dy xhat;  db = sum over rows of dy
-// All sums are fp32.  z is rebuilt from x, residual and the mask in the backward pass: storing it would move the same bytes (one write
+// Sums of eight are fp32, a thread's chunks of a row add up in fp64 (a row may have 2^28 columns, 2^17 chunks a thread), threads in fp32.  z is rebuilt from x, residual and the mask in the backward pass: storing it would move the same bytes (one write
 // and one read against two reads for one), round it, and hold one more tensor.
 #include "norm.hpp"
 
@@ -46,25 +46,32 @@ __global__ __launch_bounds__(256) void norm_wide_fwd_kernel(NormArgs a) {
   DropKey key{};
   if (RES) key = drop_key(a.drop);
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    float s = 0.0f, d = 0.0f, z[8];
+    double s64 = 0.0, d64 = 0.0;              // a thread's chunks add up in 64 bits
+    float z[8];
     Keep8 m;
     for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
       const int nv = (int)min(8ll, a.cols - c);
       load_z<TX, TR, RES>(a, key, row, c, nv, z, m);
+      float t = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s += j < nv ? z[j] : 0.0f;
+      for (int j = 0; j < 8; ++j) t += j < nv ? z[j] : 0.0f;
+      s64 += t;
     }
-    const float mean = block_sum(s, sm) / (float)a.cols;
-    s = 0.0f;
+    const float mean = block_sum((float)s64, sm) / (float)a.cols;
+    s64 = 0.0;
     for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
       const int nv = (int)min(8ll, a.cols - c);
       load_z<TX, TR, RES>(a, key, row, c, nv, z, m);
+      float t = 0.0f, u = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        s += j < nv ? (z[j] - mean) * (z[j] - mean) : 0.0f;
-        d += j < nv ? z[j] - mean : 0.0f;
+        t += j < nv ? (z[j] - mean) * (z[j] - mean) : 0.0f;
+        u += j < nv ? z[j] - mean : 0.0f;
       }
+      s64 += t;
+      d64 += u;
     }
+    float s = (float)s64, d = (float)d64;
     block_sum2(s, d, sm2);
     d /= (float)a.cols;                       // corrects the mean (norm.hpp)
     const float rstd = rsqrt_newton(norm_variance(s / (float)a.cols, d) + a.eps);
@@ -94,7 +101,8 @@ __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
   if (RES) key = drop_key(a.drop);
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const float mean = a.mean[row], rstd = a.rstd[row];
-    float s1 = 0.0f, s2 = 0.0f, z[8], w[8];
+    double s1 = 0.0, s2 = 0.0;
+    float z[8], w[8];
     Keep8 m;
     for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
       const int nv = (int)min(8ll, a.cols - c);
@@ -102,14 +110,17 @@ __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
       load_param_some<TX>(a.weight, a.p_f32, c, nv, 1.0f, w);
       Vec8<TR> d;
       load_nv(d, reinterpret_cast<const TR*>(a.dy) + row * a.ld_dy + c, nv);
+      float t = 0.0f, u = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float g = d.get(j) * w[j];
-        s1 += j < nv ? g : 0.0f;
-        s2 += j < nv ? g * ((z[j] - mean) * rstd) : 0.0f;
+        t += j < nv ? g : 0.0f;
+        u += j < nv ? g * ((z[j] - mean) * rstd) : 0.0f;
       }
+      s1 += t;
+      s2 += u;
     }
-    const float c1 = block_sum(s1, sm[0]) / (float)a.cols, c2 = block_sum(s2, sm[1]) / (float)a.cols;
+    const float c1 = block_sum((float)s1, sm[0]) / (float)a.cols, c2 = block_sum((float)s2, sm[1]) / (float)a.cols;
     for (long long c = threadIdx.x * 8; c < a.cols; c += 2048) {
       const int nv = (int)min(8ll, a.cols - c);
       const bool drop = load_z<TX, TR, RES>(a, key, row, c, nv, z, m);

@@ -754,7 +754,7 @@ def test_block_of_the_tracker_trains():
 
 # ---------------------------------------------------------------------------------------------- rows far from zero
 
-def offset_bounds(o, eps, dtype):
+def offset_bounds(o, eps, dtype, depth=None):
     """Tolerances where the mean is far larger than the spread (types: all `dtype`, parameters fp32, z exact in fp32).  depth as above.
     The first mean is off by delta <= e (depth + 2) mean|z|; the deviations from it are off by e of themselves; their mean, by which they are
     corrected, by e (depth + 3) mean|z - first| <= e (depth + 3) (delta + MAD); the variance by e (depth + 8) (var + delta^2).  So
@@ -762,7 +762,7 @@ def offset_bounds(o, eps, dtype):
     of which only e^2 mean|z| grows with the offset.  The backward pass takes z from the stored mean, an fp32 number:
       Eb = E + e |mean| rstd,  and from there the module's formulas."""
     D = o["z"].shape[-1]
-    depth = 8 * math.ceil(D / 2048) + 32
+    depth = depth or 8 * math.ceil(D / 2048) + 32
     mean = lambda t: t.mean(-1, keepdim=True)        # noqa: E731
     dev = (o["z"] - o["mean"]).abs()
     delta = E32 * (depth + 2) * mean(o["z"].abs())
@@ -1010,3 +1010,30 @@ def test_negative_views():
     assert all(torch.equal(p, q) for p, q in zip(*results))
     leaf = plain[0].detach().requires_grad_()
     assert torch.equal(torch.autograd.grad(dropout(leaf, 0.4, 3), leaf, dy)[0], dropout(dy.resolve_neg(), 0.4, 3))
+
+
+# ---------------------------------------------------------------------------------------------- very long sums
+
+@gpu
+@pytest.mark.parametrize("joined", [False, True])
+@pytest.mark.parametrize("offset", [0.0, 500.0])
+def test_norm_sums_of_millions_of_columns(offset, joined):
+    """Equal terms round alike, so that a long chain of fp32 additions drifts instead of averaging out: rows of +-1.0001, dy of 1.0003.  A sum's fp32
+    additions are eight of a chunk, a tree over 64 lanes and four waves: depth 32, however long the row is."""
+    cols = 4_000_003
+    x = (torch.arange(cols) % 2 * 2 - 1).float()[None] * torch.tensor([[1.0001], [0.7003]]) + offset
+    dy = torch.full((2, cols), 1.0003)
+    dy[:, ::3] = 0.5001
+    r = x / 2 if joined else None
+    x = x / 2 if joined else x                                                         # the join adds the halves up again, exactly
+    want = ref.norm(x, None, None, 1e-5, r, None, dy)
+    tol = offset_bounds(want, 1e-5, F32, depth=32)
+    r = None if r is None else r.cuda()
+    y, mean, rstd = hip.norm_forward(x.cuda(), None, None, 1e-5, r, want_stats=True)
+    within(mean[:, None], want["mean"], tol["mean"], "mean")
+    within(rstd[:, None], want["rstd"], tol["rstd"], "rstd")
+    within(y, want["y"], tol["y"], "y")
+    dx, dres, _, _ = hip.norm_backward(dy.cuda(), x.cuda(), mean, rstd, None, None, 1e-5, r)
+    within(dx, want["dx"], tol["dx"], "dx")
+    if joined:
+        within(dres, want["dresidual"], tol["dresidual"], "dresidual")
