@@ -146,7 +146,8 @@ __global__ __launch_bounds__(256) void norm_wide_dx_kernel(NormArgs a) {
   }
 }
 
-// partial[g][0 / 1][cols]: sums of dy xhat and of dy over the rows g, g + G, ...; a thread owns eight columns
+// partial[g][0 / 1][cols]: sums of dy xhat and of dy over the rows g, g + G, ...; a thread owns eight columns.  The wider the rows, the fewer partial
+// sums there are (one from 2 million columns on), so 64 rows add up in fp32 and these sums in fp64.
 template <class TX, class TR, int RES>
 __global__ __launch_bounds__(256) void norm_wide_dw_kernel(NormArgs a) {
   DropKey key{};
@@ -154,9 +155,23 @@ __global__ __launch_bounds__(256) void norm_wide_dw_kernel(NormArgs a) {
   const long long c = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;
   if (c >= a.cols) return;
   const int nv = (int)min(8ll, a.cols - c);
+  double dw64[8] = {}, db64[8] = {};
   float dw[8] = {}, db[8] = {}, z[8];
+  const auto flush = [&] {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      dw64[j] += dw[j];
+      db64[j] += db[j];
+      dw[j] = db[j] = 0.0f;
+    }
+  };
   Keep8 m;
+  int left = 64;
   for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    if (left-- == 0) {
+      flush();
+      left = 63;
+    }
     const float mean = a.mean[row], rstd = a.rstd[row];
     load_z<TX, TR, RES>(a, key, row, c, nv, z, m);
     Vec8<TR> d;
@@ -167,10 +182,11 @@ __global__ __launch_bounds__(256) void norm_wide_dw_kernel(NormArgs a) {
       db[j] += d.get(j);
     }
   }
+  flush();
   float* p = a.workspace + (long long)blockIdx.y * 2 * a.cols + c;
   for (int j = 0; j < nv; ++j) {
-    p[j] = dw[j];
-    p[a.cols + j] = db[j];
+    p[j] = (float)dw64[j];
+    p[a.cols + j] = (float)db64[j];
   }
 }
 

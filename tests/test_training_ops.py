@@ -1037,3 +1037,22 @@ def test_norm_sums_of_millions_of_columns(offset, joined):
     within(dx, want["dx"], tol["dx"], "dx")
     if joined:
         within(dres, want["dresidual"], tol["dresidual"], "dresidual")
+
+
+@gpu
+@pytest.mark.parametrize("cols,rows", [(16392, 200003), (2_100_001, 1603)])
+def test_norm_wide_column_sums_of_many_rows(cols, rows):
+    """Equal terms again: every row the same, dy of 1.0003 and xhat near 0.7.  A column's fp32 additions are at most 64 rows in a thread and 64 partial
+    sums (32 slices of at most 32); what 64 rows make is added up in fp64."""
+    torch.cuda.empty_cache()
+    x = torch.empty(rows, cols, device="cuda", dtype=F16)
+    x.copy_((torch.arange(cols, device="cuda") % 7 * 0.03 + 0.9).half().expand(rows, cols))
+    dy = torch.full((rows, cols), 1.0003, device="cuda").half() if rows * cols < 1 << 30 else torch.empty(rows, cols, device="cuda", dtype=F16).fill_(1.0003)
+    mean, rstd = torch.full((rows,), 0.25, device="cuda"), torch.full((rows,), 0.8001, device="cuda")
+    w = torch.ones(cols, device="cuda")
+    _, _, dw, db = hip.norm_backward(dy, x, mean, rstd, w, w, want=(False, False, True, True))
+    d, xhat = dy[0].double().cpu(), (x[0].double().cpu() - 0.25) * rstd[0].double().cpu()
+    del x, dy
+    torch.cuda.empty_cache()
+    within(dw, rows * d * xhat, E32 * (64 + 64 + 6) * rows * d * xhat, "dweight")
+    within(db, rows * d, E32 * (64 + 64 + 2) * rows * d, "dbias")
