@@ -12,9 +12,10 @@ int norm_wide_parts(long long rows, long long cols);
 int norm_finish(const NormArgs& a, int parts, hipStream_t stream);     // workspace [parts][2][cols] -> dweight, dbias
 
 // ---- teams: the threads that share a row ------------------------------------------------------------------------------
-// Thread tl of a team of T threads holds the 8-element chunks tl, T + tl, ... (K of them) of its row in registers.  Rows up to 2048
-// columns belong to a power of two of lanes of one wave with K <= 4: of the pairs (T, K) that hold the row the one with the fewest
-// T * K chunks (a lane past the row's end costs as much as one inside), the larger T among equals.  Longer rows belong to a workgroup.
+// Thread tl of a team of T threads holds the 8-element chunks tl, T + tl, ... (K of them) of its row in registers.  Rows up to 1536
+// columns (layer_norm's forward pass: 2048) belong to a power of two of lanes of one wave: of the pairs (T, K) with K <= 4 that hold the row the
+// one with the fewest T * K chunks (a lane past the row's end costs as much as one inside), the larger T among equals, so that K = 4 is left
+// for more than 192 chunks.  Longer rows belong to a workgroup.
 struct NormShape {
   int k;            // chunks a thread
   int shift;        // log2 of the lanes of a team (rows of a wave)

@@ -205,7 +205,7 @@ __global__ __launch_bounds__(AHEAD ? 512 : 1024) void norm_bwd_block_kernel(Norm
   for (int k = 0; k < K; ++k) {
     float w[8];
     sp[k] = Span::of<MODE>((k * lanes + tl) * 8, cols, k == K - 1);
-    load_param<TX, MODE == kShort ? kShort : kPlain>(a.weight, a.p_f32, sp[k], 1.0f, w);
+    load_param<TX, kPlain>(a.weight, a.p_f32, sp[k], 1.0f, w);
 #pragma unroll
     for (int j = 0; j < 8; ++j) wlds[(k * lanes + tl) * 8 + j] = w[j];      // read by this thread only
   }
@@ -218,9 +218,9 @@ __global__ __launch_bounds__(AHEAD ? 512 : 1024) void norm_bwd_block_kernel(Norm
     in.rstd = a.rstd[row];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      in.d[k].template load<MODE>(pd + sp[k].at, 8 - sp[k].cut);
-      in.x[k].template load<MODE>(px + sp[k].at, 8 - sp[k].cut);
-      if (RES) in.r[k].template load<MODE>(pr + sp[k].at, 8 - sp[k].cut);
+      in.d[k].template load<MODE>(pd + sp[k].at);
+      in.x[k].template load<MODE>(px + sp[k].at);
+      if (RES) in.r[k].template load<MODE>(pr + sp[k].at);
     }
   };
   if (AHEAD && blockIdx.x < a.rows) load(blockIdx.x);
@@ -330,8 +330,7 @@ template <class TX, class TR, int RES, LoadMode MODE> static int backward_rows(c
   else if (sh.block) norm_bwd_block_kernel<TX, TR, RES, 2, false, MODE><<<grid, sh.threads, lds, s>>>(a);
   else if (sh.k == 1) norm_bwd_kernel<TX, TR, RES, 1, MODE><<<grid, kBwdThreads, 0, s>>>(a, sh.shift);
   else if (sh.k == 2) norm_bwd_kernel<TX, TR, RES, 2, MODE><<<grid, kBwdThreads, 0, s>>>(a, sh.shift);
-  else if (sh.k == 3) norm_bwd_kernel<TX, TR, RES, 3, MODE><<<grid, kBwdThreads, 0, s>>>(a, sh.shift);
-  else norm_bwd_kernel<TX, TR, RES, 4, MODE><<<grid, kBwdThreads, 0, s>>>(a, sh.shift);
+  else norm_bwd_kernel<TX, TR, RES, 3, MODE><<<grid, kBwdThreads, 0, s>>>(a, sh.shift);
   if (check_launch("norm_backward")) return -1;
   if (grid > 1 && (a.dweight != nullptr || a.dbias != nullptr)) return norm_finish(a, grid, s);
   return 0;

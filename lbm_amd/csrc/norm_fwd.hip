@@ -136,16 +136,16 @@ __global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
     const TR* pr = reinterpret_cast<const TR*>(a.residual) + row * a.ld_r;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      in.x[k].template load<MODE>(px + sp[k].at, 8 - sp[k].cut);
-      if (RES) in.r[k].template load<MODE>(pr + sp[k].at, 8 - sp[k].cut);
+      in.x[k].template load<MODE>(px + sp[k].at);
+      if (RES) in.r[k].template load<MODE>(pr + sp[k].at);
     }
   };
   float w[K][8], b[K][8];
   load(blockIdx.x);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    load_param<TX, MODE == kShort ? kShort : kPlain>(a.weight, a.p_f32, sp[k], 1.0f, w[k]);
-    load_param<TX, MODE == kShort ? kShort : kPlain>(a.bias, a.p_f32, sp[k], 0.0f, b[k]);
+    load_param<TX, kPlain>(a.weight, a.p_f32, sp[k], 1.0f, w[k]);
+    load_param<TX, kPlain>(a.bias, a.p_f32, sp[k], 0.0f, b[k]);
   }
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     float z[K][8];
@@ -190,10 +190,12 @@ template <class TX, class TR, int RES, LoadMode MODE> static int forward_rows(co
     return check_launch("norm_forward");
   }
   constexpr int U1 = RES ? 2 : 4, U2 = RES ? 1 : 2;
-  if (sh.k == 4) return wave_forward<TX, TR, RES, 4, 1, MODE>(a, sh, s);
+  if constexpr (RES == 0)
+    if (sh.k == 4) return wave_forward<TX, TR, RES, 4, 1, MODE>(a, sh, s);
   const bool many = a.rows >= (long long)sh.teams() * (sh.k == 1 ? U1 : U2) * kManyGroups;
   if (sh.k == 1) return many ? wave_forward<TX, TR, RES, 1, U1, MODE>(a, sh, s) : wave_forward<TX, TR, RES, 1, 1, MODE>(a, sh, s);
-  if (sh.k == 2) return many ? wave_forward<TX, TR, RES, 2, U2, MODE>(a, sh, s) : wave_forward<TX, TR, RES, 2, 1, MODE>(a, sh, s);
+  if constexpr (RES == 0 || MODE != kOdd)      // the join's two chunks a lane are always loaded plainly (below)
+    if (sh.k == 2) return many ? wave_forward<TX, TR, RES, 2, U2, MODE>(a, sh, s) : wave_forward<TX, TR, RES, 2, 1, MODE>(a, sh, s);
   return many ? wave_forward<TX, TR, RES, 3, U2, MODE>(a, sh, s) : wave_forward<TX, TR, RES, 3, 1, MODE>(a, sh, s);
 }
 template <class TX, class TR, int RES> static int forward(const NormArgs& a, hipStream_t s) {

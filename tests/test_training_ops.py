@@ -1056,3 +1056,18 @@ def test_norm_wide_column_sums_of_many_rows(cols, rows):
     torch.cuda.empty_cache()
     within(dw, rows * d * xhat, E32 * (64 + 64 + 6) * rows * d * xhat, "dweight")
     within(db, rows * d, E32 * (64 + 64 + 2) * rows * d, "dbias")
+
+
+def test_no_kernel_that_no_call_reaches():
+    """Teams of a wave hold four chunks a lane only in layer_norm's forward pass (1537 .. 2048 columns), and the join's two chunks a lane are never loaded
+    dword by dword: kernels for the other cases would only make the library larger."""
+    import os
+    import re
+    blob = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "lbm_amd", "liblbm_hip.so"), "rb").read()
+    found = {m.group(0) for m in re.finditer(rb"_ZN3lbm15norm_(bwd|fwd)_kernelI[A-Za-z0-9_]+NS_8LoadModeE[0-9]EEEv", blob)}
+    assert len(found) > 40
+    fwd = [m for m in found if b"norm_fwd" in m]
+    for m in found - set(fwd):
+        assert not re.search(rb"Li4ELNS_8LoadMode", m), m                              # <TX, TR, RES, K, MODE>
+    for m in fwd:                                                                      # <TX, TR, RES, K, U, MODE>
+        assert not re.search(rb"Li1ELi4ELi\dELNS_8LoadMode", m) and not re.search(rb"Li1ELi2ELi\dELNS_8LoadModeE1E", m), m
