@@ -1071,3 +1071,50 @@ def test_no_kernel_that_no_call_reaches():
         assert not re.search(rb"Li4ELNS_8LoadMode", m), m                              # <TX, TR, RES, K, MODE>
     for m in fwd:                                                                      # <TX, TR, RES, K, U, MODE>
         assert not re.search(rb"Li1ELi4ELi\dELNS_8LoadMode", m) and not re.search(rb"Li1ELi2ELi\dELNS_8LoadModeE1E", m), m
+
+
+# ---------------------------------------------------------------------------------------------- several rows a team, a workgroup, a launch
+
+MANY = [  # rows just above a threshold and no multiple of it; columns; types
+    # forward in a wave: four (K = 1) and two (K = 2, 3) rows in flight a team, from teams * U * 2048 rows on; backward: 16 rounds of a workgroup
+    (65536 + 13, 256, (F16, None, F32)), (65536 + 13, 253, (BF16, None, BF16)), (131072 + 5, 136, (F32, None, F32)), (131072 + 5, 135, (F16, None, F16)),
+    (16384 + 3, 1000, (BF16, None, F32)), (16384 + 3, 1001, (F16, None, F32)), (16384 + 5, 1048, (F16, None, F32)), (5000, 2047, (BF16, None, F32)),
+    (32768 + 9, 250, (F16, F32, F32)), (32768 + 9, 249, (BF16, BF16, BF16)), (9001, 1021, (F16, F16, F32)), (6000, 1536, (BF16, F32, F32)), (262144 + 77, 5, (F16, F32, F32)),
+    # forward in a workgroup: more than 256 (1024 / threads) rows, so that a second and a third row meet the loads ahead and the sums' memory;
+    # backward: more than two rows a workgroup, one, two (rows >= 4096) and three (>= 6144) workgroups a CU
+    (1300, 2051, (F16, None, F32)), (2900, 2051, (F32, F32, F32)), (4200, 2051, (BF16, BF16, F32)), (6200, 1537, (BF16, None, F32)), (6200, 1544, (F16, F32, F32)),
+    (800, 4104, (F32, None, F32)), (1101, 4099, (BF16, BF16, BF16)), (600, 8192, (F16, None, F16)), (821, 8191, (BF16, F32, F32)),
+    (600, 16384, (BF16, None, F32)), (777, 16383, (F16, None, F32)), (600, 16384, (F32, None, F32)), (600, 16377, (F16, F16, F32)), (520, 9000, (F32, F32, F32)),
+    # beyond 16384 columns: several rounds of a workgroup in the column sums
+    (1100, 17001, (BF16, F32, F32)),
+]
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols,types", MANY, ids=lambda v: "-".join(str(d)[6:] for d in v) if isinstance(v, tuple) else str(v))
+def test_norm_many_rows_against_float64(rows, cols, types):
+    check(operands((rows, cols), *types, "both", seed=rows + cols), p=0.15, seed=rows, offset=cols)
+
+
+@gpu
+@pytest.mark.parametrize("cols", [256, 257, 2051, 20001])
+def test_norm_column_sums_beyond_32_bit_indexes(cols):
+    """4.4e9 elements: dy is zero but in a few rows at both ends and around 2^31 and 2^32 elements, so that the oracle's sums are short."""
+    rows, p, seed, offset = 4_400_000_000 // cols, 0.3, 99, 5
+    torch.cuda.empty_cache()
+    g = torch.Generator("cuda").manual_seed(cols)
+    x = torch.empty(rows, cols, device="cuda", dtype=F16).normal_(generator=g)
+    dy = torch.zeros(rows, cols, device="cuda", dtype=F16)
+    at = [0, 1, 2 ** 31 // cols - 1, 2 ** 31 // cols, 2 ** 32 // cols - 1, 2 ** 32 // cols, 2 ** 32 // cols + 1, rows - 2, rows - 1]
+    for r in at:
+        dy[r] = torch.randn(cols, device="cuda", generator=g).half()
+    w = torch.randn(cols, device="cuda", generator=g)
+    _, mean, rstd = hip.norm_forward(x, w, w, 1e-5, x, p, seed, offset, want_stats=True)
+    _, _, dw, db = hip.norm_backward(dy, x, mean, rstd, w, w, 1e-5, x, p, seed, offset, want=(False, False, True, True))
+    factor = torch.cat([ref.keep((1, cols), p, seed, offset, first=r * cols) for r in at]).double() * ref.scale(p)
+    want = ref.norm(x[at], w, w, 1e-5, x[at], factor, dy[at])
+    tol = bounds(want, 1e-5, F16, F16, F32, ref.scale(p))
+    within(dw, want["dweight"], tol["dweight"], "dweight")
+    within(db, want["dbias"], tol["dbias"], "dbias")
+    del x, dy
+    torch.cuda.empty_cache()
