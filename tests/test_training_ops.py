@@ -1118,3 +1118,21 @@ def test_norm_column_sums_beyond_32_bit_indexes(cols):
     within(db, want["dbias"], tol["dbias"], "dbias")
     del x, dy
     torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------------------------------------- the build
+
+def _plan(*args):
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "lbm_amd", "csrc")
+    return subprocess.run(["make", "-n", "-C", csrc, *args], check=True, capture_output=True, text=True).stdout
+
+
+def test_the_library_builds_without_torch():
+    """The C interface needs no torch: only the host path of the training operators is left out, and make says so."""
+    with_torch, without = _plan("-B", "all"), _plan("-B", "all", "PYTHON=/bin/false")
+    assert "torch_ops.cpp" in with_torch and "is not built" not in with_torch
+    assert "torch_ops.cpp" not in without and "is not built" in without
+    for plan in (with_torch, without):
+        assert "norm_bwd.hip" in plan and "-o ../liblbm_hip.so" in plan
