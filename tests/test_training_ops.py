@@ -1136,3 +1136,9 @@ def test_the_library_builds_without_torch():
     assert "torch_ops.cpp" not in without and "is not built" in without
     for plan in (with_torch, without):
         assert "norm_bwd.hip" in plan and "-o ../liblbm_hip.so" in plan
+
+
+def test_the_host_path_is_rebuilt_for_another_torch():
+    import os
+    version = os.path.join(os.path.dirname(torch.__file__), "version.py")
+    assert "torch_ops.cpp" in _plan("-W", version, "all")
