@@ -1142,3 +1142,16 @@ def test_the_host_path_is_rebuilt_for_another_torch():
     import os
     version = os.path.join(os.path.dirname(torch.__file__), "version.py")
     assert "torch_ops.cpp" in _plan("-W", version, "all")
+
+
+def test_build_compiles_what_is_built_already(monkeypatch):
+    """build() is the check that every source compiles: it may not stop at a library that is there."""
+    import subprocess
+
+    import __graft_entry__ as entry
+    calls = []
+    monkeypatch.setattr(subprocess, "run", lambda cmd, **kw: calls.append(cmd))
+    entry.build()
+    monkeypatch.undo()
+    plan = subprocess.run([*calls[0], "-n"], check=True, capture_output=True, text=True).stdout
+    assert "norm_bwd.hip" in plan and "gemm.hip" in plan and "torch_ops.cpp" in plan
