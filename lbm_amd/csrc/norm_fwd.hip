@@ -167,8 +167,11 @@ __global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
   }
 }
 
-// Rows in flight a team: four (the join two) when that still makes 2048 workgroups, else one (65536 x 256 f16: 14.3 us with four, 15.8 with
-// one; the join at 9216 x 256: 9.0 us with four, 6.9 with one).
+// Rows in flight a team when that still makes 2048 workgroups, else one:
+//   layer_norm   four, with two or three chunks a lane two: 65536 x 256 f16 14.8 us with four, 16.1 with one (9216 x 256: 5.7 and 4.4); 65536 x 1000 bf16
+//                52.8 us with two, 56.6 with one (8192 x 1000: the same)
+//   the join     two where its rows are no multiple of eight, whose masks wait for other lanes: 400000 x 249 bf16 139 us with two, 152 with one; other rows
+//                one, which leaves more waves: 131072 x 256 bf16 37.4 us with one, 40.3 with two, 2000000 x 64 f16 137 and 147, fp32 residuals the same
 constexpr long long kManyGroups = 2048;
 // Chunks that a wave may hold: the join's four a lane leave two waves a SIMD (93750 x 1600 bf16: 218 us, 181 in a workgroup), three do not
 // (97656 x 1536: 156 us, 179 in a workgroup).
@@ -192,7 +195,7 @@ template <class TX, class TR, int RES, LoadMode MODE> static int forward_rows(co
   constexpr int U1 = RES ? 2 : 4, U2 = RES ? 1 : 2;
   if constexpr (RES == 0)
     if (sh.k == 4) return wave_forward<TX, TR, RES, 4, 1, MODE>(a, sh, s);
-  const bool many = a.rows >= (long long)sh.teams() * (sh.k == 1 ? U1 : U2) * kManyGroups;
+  const bool many = a.rows >= (long long)sh.teams() * (sh.k == 1 ? U1 : U2) * kManyGroups && (RES == 0 || (a.cols & 7) != 0);
   if (sh.k == 1) return many ? wave_forward<TX, TR, RES, 1, U1, MODE>(a, sh, s) : wave_forward<TX, TR, RES, 1, 1, MODE>(a, sh, s);
   if constexpr (RES == 0 || MODE != kOdd)      // the join's two chunks a lane are always loaded plainly (below)
     if (sh.k == 2) return many ? wave_forward<TX, TR, RES, 2, U2, MODE>(a, sh, s) : wave_forward<TX, TR, RES, 2, 1, MODE>(a, sh, s);
