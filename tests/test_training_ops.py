@@ -1155,3 +1155,12 @@ def test_build_compiles_what_is_built_already(monkeypatch):
     monkeypatch.undo()
     plan = subprocess.run([*calls[0], "-n"], check=True, capture_output=True, text=True).stdout
     assert "norm_bwd.hip" in plan and "gemm.hip" in plan and "torch_ops.cpp" in plan
+
+
+@gpu
+def test_batched_gradients_are_refused():
+    """is_grads_batched maps the backward pass with vmap: gradients without memory of their own."""
+    x, w = torch.randn(5, 24, device="cuda").requires_grad_(), torch.ones(24, device="cuda").requires_grad_()
+    for y in (layer_norm(x, w), dropout(x, 0.5, 1), dropout_add_layer_norm(x, x.detach(), w, p=0.5, seed=torch.tensor([4], device="cuda"))):
+        with pytest.raises(hip.HipError, match="plain dense tensor"):
+            torch.autograd.grad(y, x, torch.ones(2, 5, 24, device="cuda"), is_grads_batched=True)
