@@ -93,8 +93,7 @@ __device__ __forceinline__ float rsqrt_newton(float v) {
 // What is left grows with the spread and with e^2 |m|.  Both sums are exact enough for d^2 as long as the variance is not far below it; where it is
 // (a constant row), the difference is rounding noise and 2^-18 of the squares stands for it, so that no eps makes a result of that noise.
 __device__ __forceinline__ float norm_variance(float squares, float d) {
-  const float v = fmaf(-d, d, squares), least = squares * 0x1p-18f;
-  return v > least ? v : least;              // NaN and infinity come through `least`
+  return fmaxf(fmaf(-d, d, squares), squares * 0x1p-18f);      // NaN and infinity come through the second
 }
 
 // a * b rounded by itself: contracted into the subtractions, m would be another number in z - m than in m + d
@@ -123,6 +122,41 @@ __device__ __forceinline__ float lanes_sum(float v, int shift) {
   }
   for (int s = 1; s < 1 << shift; s <<= 1) v += __shfl_xor(v, s);
   return v;
+}
+// two sums in one go: a step of one fills the wait between two of the other
+__device__ __forceinline__ void lanes_sum2(float& u, float& v, int shift) {
+  if (shift >= 4) {
+    u = row16_sum(u);
+    v = row16_sum(v);
+    if (shift >= 5) {
+      u = lane16_sum(u);
+      v = lane16_sum(v);
+    }
+    if (shift >= 6) {
+      u = lane32_sum(u);
+      v = lane32_sum(v);
+    }
+    return;
+  }
+  for (int s = 1; s < 1 << shift; s <<= 1) {
+    u += __shfl_xor(u, s);
+    v += __shfl_xor(v, s);
+  }
+}
+// two sums behind one barrier; `sm`: 16 pairs
+__device__ __forceinline__ void block_sum2(float& u, float& v, float (*sm)[2]) {
+  lanes_sum2(u, v, 6);
+  const int nw = blockDim.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+    sm[threadIdx.x >> 6][0] = u;
+    sm[threadIdx.x >> 6][1] = v;
+  }
+  __syncthreads();
+  u = v = 0.0f;
+  for (int i = 0; i < nw; ++i) {
+    u += sm[i][0];
+    v += sm[i][1];
+  }
 }
 __device__ __forceinline__ float wave64_sum(float v) { return lane32_sum(lane16_sum(row16_sum(v))); }
 

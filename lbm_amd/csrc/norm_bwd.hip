@@ -311,7 +311,9 @@ static int norm_parts(long long rows, long long cols, bool lean) {
   int per_cu = !sh.block ? 1 : sh.threads <= 128 ? 3 : sh.threads <= 256 ? 2 : 1;
   while (per_cu > 1 && rows < 8 * 256 * per_cu) --per_cu;      // a partial sum costs the traffic of two or three rows
   const long long g = (rows + sh.teams() - 1) / sh.teams();
-  if (g <= (sh.block || sh.k > 1 ? 2 : 4)) return 1;       // a few rounds of one workgroup (64 x 256: 6.3 us) cost less than the second launch (8.3)
+  if (g <= (sh.block || sh.k > 1 ? 2 : 4)) return 1;
+  // (a few rounds of one workgroup cost less than the second launch: 64 x 256 join 8.4 us and 8.7 with it, 2048 x 8 f32 7.1 and 9.3, 256 x 64 7.0 and 8.9, 16 x 512
+  // 4.1 and 8.3, 16 x 1000 bf16 6.1 and 8.6, 2 x 8192 bf16 5.7 and 8.6; two rows of 16384 columns of an fp32 join 17.2 and 15.4)
   return (int)std::min(g, 256ll * per_cu);
 }
 

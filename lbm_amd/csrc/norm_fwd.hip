@@ -103,9 +103,10 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift, lo
     float z[K][8];
     const float mean = product(lanes_sum(join_row<TX, TR, RES, K, false, MODE>(a, key, in[u], sp, base + r, lanes, tl, z), shift), inv);
     float d;
-    const float s = deviate<K>(z, mean, sp, d);
-    d = product(lanes_sum(d, shift), inv);
-    const float rstd = rsqrt_newton(norm_variance(lanes_sum(s, shift) * inv, d) + a.eps);
+    float s = deviate<K>(z, mean, sp, d);
+    lanes_sum2(s, d, shift);
+    d = product(d, inv);
+    const float rstd = rsqrt_newton(norm_variance(s * inv, d) + a.eps);
     if (r > last) continue;
     if (tl == 0 && a.mean != nullptr) {
       a.mean[base + r] = mean + d;
@@ -204,7 +205,8 @@ template <class TX, class TR, int RES, LoadMode MODE> static int forward_rows(co
 template <class TX, class TR, int RES> static int forward(const NormArgs& a, hipStream_t s) {
   constexpr LoadMode odd = sizeof(TX) == 2 ? kOdd : kPlain;
   if (a.cols < 8) return wave_forward<TX, TR, RES, 1, 1, kShort>(a, norm_shape(a.cols, 1), s);
-  // (the join's two chunks a lane are the exception: 146914 x 1021 bf16 184 us with plain loads, 201 dword by dword)
+  // (the join's two chunks a lane are the exception: 146914 x 1021 bf16 194 us with plain loads, 208 dword by dword; 190000 x 785 224 and 247; beside an
+  // fp32 residual 264 and 275 at 160000 x 901, the same at 100000 x 1021)
   const NormShape sh = norm_shape(a.cols, wave_chunks<RES>());
   if (odd == kOdd && (odd_rows<TX>(a.x, a.ld_x) || (RES && odd_rows<TR>(a.residual, a.ld_r))) && !(RES && !sh.block && sh.k == 2)) return forward_rows<TX, TR, RES, odd>(a, s);
   return forward_rows<TX, TR, RES, kPlain>(a, s);

@@ -308,21 +308,5 @@ __device__ __forceinline__ float block_sum(float v, float* sm) {
   for (int i = 0; i < nw; ++i) t += sm[i];
   return t;
 }
-// two sums behind one barrier; `sm`: 16 pairs
-__device__ __forceinline__ void block_sum2(float& u, float& v, float (*sm)[2]) {
-  u = wave_sum(u);
-  v = wave_sum(v);
-  const int nw = blockDim.x >> 6;
-  if ((threadIdx.x & 63) == 0) {
-    sm[threadIdx.x >> 6][0] = u;
-    sm[threadIdx.x >> 6][1] = v;
-  }
-  __syncthreads();
-  u = v = 0.0f;
-  for (int i = 0; i < nw; ++i) {
-    u += sm[i][0];
-    v += sm[i][1];
-  }
-}
 
 }  // namespace lbm
