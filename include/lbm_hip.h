@@ -95,8 +95,10 @@ int lbm_hip_dropout(const void* x, void* y, int64_t n, int32_t type, double p, u
                     lbm_stream_t stream);
 
 /* z = x (residual == NULL) or residual + dropout(x);  y = (z - mean(z)) * rstd * weight + bias per row,
- * rstd = 1 / sqrt(mean((z - mean)^2) + eps).  Statistics and sums are fp32; the forward pass corrects its mean by the mean of the
- * deviations from it, so a row far from zero loses nothing of its spread; the backward pass takes z from the stored mean, which is rounded to fp32.  Types: x and dx x_type; residual, y, dy and dresidual
+ * rstd = 1 / sqrt(mean((z - mean)^2) + eps).  Statistics and sums are fp32 (fp64 where a chain of additions grows with the sizes beyond
+ * 16384 columns).  The forward pass corrects its mean by the mean of the deviations from it: what a row far from zero loses goes by its
+ * spread.  The backward pass takes z from the stored mean, which is rounded to fp32.  A row whose sum or sum of squared deviations is beyond
+ * fp32's range gives NaN.  Types: x and dx x_type; residual, y, dy and dresidual
  * res_type (= x_type, or LBM_TYPE_F32: half-precision products beside an fp32 residual stream; without a residual = x_type);
  * weight, bias and their gradients param_type (= x_type or LBM_TYPE_F32), either may be NULL.  Element strides between rows:
  * ld_x, ld_residual, ld_dy (>= cols, < 2^31); outputs are dense and overlap no input.  1 <= cols <= 2^28.
@@ -105,7 +107,8 @@ int lbm_hip_dropout(const void* x, void* y, int64_t n, int32_t type, double p, u
  * backward: reads dy, x, residual, weight, mean, rstd; writes the non-NULL ones of dx, dresidual, dweight, dbias
  *   (g = dy * weight; dz = rstd * (g - mean(g) - xhat * mean(g * xhat)); dresidual = dz; dx = dropout's gradient of dz, or dz;
  *   dweight = sum over rows of dy * xhat, dbias = sum over rows of dy).  z is rebuilt from x, residual and the mask.
- *   workspace: lbm_hip_norm_workspace_bytes(rows, cols), 16-byte aligned, needed with dweight or dbias; its contents are not kept.
+ *   workspace: lbm_hip_norm_workspace_bytes(rows, cols), 16-byte aligned, needed with dweight or dbias; its contents are not kept, and calls
+ *   that may run at the same time (other streams, graphs replayed side by side) need one each.
  *   The sums over rows are made in an order that only the sizes decide: the same call gives the same bits.                     */
 typedef struct {
   const void* x; const void* residual; const void* weight; const void* bias;

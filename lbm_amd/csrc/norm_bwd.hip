@@ -110,7 +110,7 @@ __device__ __forceinline__ void bwd_put(const NormArgs& a, const Span (&sp)[K], 
 
 // Rows of lanes of a wave.  The next row's loads are issued when this row has become xhat and g, and pass behind its sums and stores.
 // Eight waves a workgroup, one workgroup a CU: half the partial sums of four waves and two (150000 x 1024 join 315 -> 295 us, 16320 x 257 16.4 -> 15.1).
-// Bound by HBM: 589824 x 256 bf16 173 us (5.2 TB/s), the join 271 us (5.6).  A grid that is no whole number a CU is not (640 workgroups of 256
+// Bound by HBM: 589824 x 256 bf16 173 us (5.2 TB/s), the join 277 us (5.5).  A grid that is no whole number a CU is not (640 workgroups of 256
 // threads: the join 316 us, 512: 274), nor are contiguous rows a workgroup (191 us): neighbouring workgroups on neighbouring rows.
 constexpr int kBwdThreads = 512, kBwdWaves = kBwdThreads / 64;
 template <class TX, class TR, int RES, int K, LoadMode MODE>
@@ -188,8 +188,9 @@ __global__ __launch_bounds__(kBwdThreads) void norm_bwd_kernel(NormArgs a, int s
 }
 
 // Rows of a workgroup.  AHEAD: the next row's loads pass behind this row's sums, as above, at the price of registers (512 threads at
-// most); otherwise up to 1024 threads with 128 registers each, a row at a time.  18000 x 8192 bf16 171 us (5.2 TB/s), the join 280 us (5.3; a row at a
-// time 303); 9000 x 16384 188 us (4.7: the partial sums are 7 % of the traffic), fp32 338 us (5.2).  A few long rows are bound by one
+// most); otherwise up to 1024 threads with 128 registers each, a row at a time.  18000 x 8192 bf16 165 - 184 us (4.8 - 5.4 TB/s), the join 270 - 285 us (5.2 - 5.5; a
+// row at a time 303); 9000 x 16384 188 us (4.7: the partial sums are 7 % of the traffic), fp32 338 us (5.2), the join a row at a time 285 us (5.2), f16 beside an fp32
+// residual 470 (5.0).  A few long rows are bound by one
 // row's latency after the other (4096 x 2048: 20 us, eight rows a workgroup).
 template <class TX, class TR, int RES, int K, bool AHEAD, LoadMode MODE>
 __global__ __launch_bounds__(AHEAD ? 512 : 1024) void norm_bwd_block_kernel(NormArgs a) {
@@ -257,8 +258,8 @@ __global__ __launch_bounds__(AHEAD ? 512 : 1024) void norm_bwd_block_kernel(Norm
     }
 }
 
-// dweight / dbias = the partial sums added up in a fixed order: 32 columns x 32 slices of the partial sums a workgroup.  4 - 5 us, of which
-// the launch is half.
+// dweight / dbias = the partial sums added up in a fixed order: 32 columns x 32 slices of the partial sums a workgroup.  4 - 5 us up to 8192 columns, 7 at
+// 16384: latencies (8 dependent rounds of loads, a barrier, 32 reads), not bandwidth.
 template <class T>
 __global__ __launch_bounds__(1024) void norm_finish_kernel(const float* part, int parts, long long cols, T* dweight, T* dbias) {
   __shared__ float sm[32][33];

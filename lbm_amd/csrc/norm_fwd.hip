@@ -65,8 +65,8 @@ template <class TR> __device__ __forceinline__ void put_y(TR* y, float (&z)[8], 
 }
 
 // Rows of up to 2048 columns.  U rows a team are loaded before the first is used, and a workgroup ends after them: a grid in row order
-// keeps the whole chip on neighbouring pages.  589824 x 256 bf16 107 us (5.6 TB/s), the join 158 us (5.7); 583657 x 257 134 us (4.5: the 33rd
-// chunk of a row has a stripe of its own).  Beside HBM the vector instructions are next: half of the issue slots at 256 columns.
+// keeps the whole chip on neighbouring pages.  589824 x 256 bf16 107 us (5.6 TB/s), the join 158 us (5.7); 583657 x 257 139 us (4.3: the 33rd
+// chunk of a row has a stripe of its own).  Beside HBM the vector instructions are next: 57 % of the issue slots at 256 columns.
 template <class TX, class TR, int RES, int K, int U, LoadMode MODE>
 __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift, long long first) {
   const int lanes = 1 << shift, tl = threadIdx.x & (lanes - 1), team = threadIdx.x >> shift, teams = 256 >> shift, cols = (int)a.cols;
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(NormArgs a, int shift, lo
 
 // Rows of a workgroup.  The next row's loads are issued when this row has become z, so they pass behind its two sums and its stores: with
 // 512 or 1024 threads a row only one or two rows are on a CU, and without that its memory was idle half of the time (8192 x 8192 bf16
-// 74 us, now 49: 5.5 TB/s; 9000 x 16384 110 us, 5.3).
+// 74 us, now 50: 5.4 TB/s; 9000 x 16384 114 us, 5.2).
 template <class TX, class TR, int RES, int K, LoadMode MODE>
 __global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
   __shared__ float sm[16], sm2[16][2];
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(1024) void norm_fwd_block_kernel(NormArgs a) {
 //                one, which leaves more waves: 131072 x 256 bf16 37.4 us with one, 40.3 with two, 2000000 x 64 f16 137 and 147, fp32 residuals the same
 constexpr long long kManyGroups = 2048;
 // Chunks that a wave may hold: the join's four a lane leave two waves a SIMD (93750 x 1600 bf16: 218 us, 181 in a workgroup), three do not
-// (97656 x 1536: 156 us, 179 in a workgroup).
+// (97656 x 1536: 166 us, 178 in a workgroup; f16 beside an fp32 residual 261 and 284).
 template <int RES> constexpr int wave_chunks() { return RES ? 192 : 256; }
 template <class TX, class TR, int RES, int K, int U, LoadMode MODE> static int wave_forward(const NormArgs& a, const NormShape& sh, hipStream_t s) {
   const long long per = (long long)sh.teams() * U, most = grid_most(256) * per;

@@ -1,6 +1,7 @@
 // Layer normalisation of rows beyond what a workgroup holds in registers, of any length, forward and backward: a workgroup walks a row in
 // several sweeps (the later ones find it in L2) and the gradients of weight and bias are summed by a kernel of their own that owns
-// columns.  8000 x 20000 bf16 209 us forward (3.1 TB/s of x and y), 415 us backward (2.3): three sweeps over a row instead of one.
+// columns.  8000 x 20000 bf16 210 us forward (3.0 TB/s of x and y), 416 us backward (2.3), the join 332 and 666 (2.9, 2.4): three sweeps over a row
+// instead of one.
 //   z = residual + dropout(x);  m = mean(z);  v = mean((z - m)^2) (norm_variance);  rstd = 1 / sqrt(v + eps);  xhat = (z - m) rstd;  y = xhat w + b
 //   g = dy w;  dz = rstd (g - mean(g) - xhat mean(g xhat));  dresidual = dz;  dx = keep ? dz scale : 0
 //   dw = sum over rows of dy xhat;  db = sum over rows of dy

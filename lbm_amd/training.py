@@ -16,7 +16,8 @@ when it is replayed, so advancing it in place draws new masks; between a forward
 
 There is no CPU path, and no automatic type conversion under ``torch.autocast``: x and residual are taken in the types they have.
 The host path -- checks, outputs, autograd nodes -- is C++ (csrc/torch_ops.cpp): in a step of the tracker's sizes it is what these calls cost.
-The gradients of the two normalisations are not differentiable themselves (refused); dropout's are.
+The gradients of the two normalisations are not differentiable themselves (refused); dropout's are.  ``torch.func`` transforms (``vmap``, ``grad``),
+batched gradients and sparse tensors are refused; ``torch.compile`` runs the operators as they are, outside of its graphs.
 """
 from __future__ import annotations
 
@@ -34,14 +35,15 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
     x (..., D): rows of the last dimension at one stride are read where they lie (a slice of a merged projection), any other
     layout is copied first.  weight / bias (D,): x's type or float32, both the same; either may be None.  The result is dense.
-    A row whose squared deviations add up beyond fp32's range (3.4e38) gives NaN."""
+    A row whose sum or sum of squared deviations is beyond fp32's range (3.4e38) gives NaN."""
     return hip.ops().norm(x, None, weight, bias, eps, 0.0, 0, None, 0)
 
 
 def dropout(x: torch.Tensor, p: float, seed: Seed, offset: int = 0) -> torch.Tensor:
     """``x / (1 - p)`` where the mask of (seed, offset) keeps an element, 0 elsewhere -- whatever the dropped value was, NaN included.
 
-    p is taken to the nearest multiple of 2^-32 (0: a plain copy; 1: all zeros).  The result is dense, in x's type."""
+    p is taken to the nearest multiple of 2^-32 (0: a plain copy; 1: all zeros).  The result is dense, in x's type; an x that is not dense
+    (a slice's rows included) is copied first."""
     return hip.ops().dropout(x, *hip._drop_args(p, seed, offset))
 
 

@@ -76,7 +76,8 @@ if __name__ == "__main__":
     else:
         for a in [(8, 256), (1024, 256), (65536, 256, "f16"), (589824, 256, "bf16"), (589824, 256, "f32"), (16320, 257, "bf16"), (146914, 1021, "f16"), (8192, 8192, "bf16"),
                   (9000, 16384, "bf16"), (8000, 20000, "bf16"), (64, 256, "f32", "f32"), (9216, 256, "f16", "f32"), (4099, 1537, "bf16", "bf16"), (589824, 256, "bf16", "bf16"),
-                  (150000, 1024, "bf16", "bf16"), (148000, 1021, "f16", "f16"), (36000, 4096, "bf16", "bf16")]:
+                  (589824, 256, "f32", "f32"), (589824, 256, "f16", "f32"), (589824, 256, "bf16", "f32"), (150000, 1024, "bf16", "bf16"), (148000, 1021, "f16", "f16"),
+                  (36000, 4096, "bf16", "bf16"), (18000, 8192, "bf16", "bf16"), (9000, 16384, "bf16", "bf16"), (9000, 16384, "f16", "f32"), (8000, 20000, "bf16", "bf16")]:
             norm(*a)
         for a in [(1 << 20, "f32"), (9217 * 1021, "f16"), (65536 * 1024, "bf16"), (589824 * 256, "f32"), (589824 * 256, "bf16")]:
             drop(*a)

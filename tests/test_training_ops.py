@@ -1164,3 +1164,20 @@ def test_batched_gradients_are_refused():
     for y in (layer_norm(x, w), dropout(x, 0.5, 1), dropout_add_layer_norm(x, x.detach(), w, p=0.5, seed=torch.tensor([4], device="cuda"))):
         with pytest.raises(hip.HipError, match="plain dense tensor"):
             torch.autograd.grad(y, x, torch.ones(2, 5, 24, device="cuda"), is_grads_batched=True)
+
+
+@gpu
+@pytest.mark.filterwarnings("ignore")
+def test_inside_a_compiled_function():
+    """torch.compile leaves the operators outside of its graphs: the same bits, gradients too."""
+    o = operands((40, 136), F32, F32, F32, "both", seed=41)
+
+    def block(x, r, w, b):
+        return layer_norm(torch.sin(dropout_add_layer_norm(dropout(x * 2, 0.2, 5, 1), r, w, b, p=0.3, seed=5, offset=2)) + r, w, b)
+
+    results = []
+    for f in (block, torch.compile(block, backend="eager")):
+        t = [o[k].detach().clone().requires_grad_() for k in ("x", "residual", "weight", "bias")]
+        y = f(*t)
+        results.append([y.detach(), *torch.autograd.grad(y, t, o["dy"])])
+    assert all(torch.equal(p, q) for p, q in zip(*results))
