@@ -241,6 +241,20 @@ Tensor run_dropout(const Tensor& x, const Drop& drop) {
 // ---- autograd --------------------------------------------------------------------------------------------------------
 SavedVariable saved(const Tensor& t) { return SavedVariable(t, /*is_output=*/false); }
 
+// A captured backward pass that would run on into an eager graph on the default stream: that stream cannot wait inside the capture, and the
+// process would end there.  Asked before the node hands its gradients on; the engine has made the node's stream the current one.
+void refuse_captured_into_eager(const char* what, Node& node, const std::vector<bool>& wanted) {
+  const auto mine = node.stream();
+  if (!mine.has_value() || mine->id() == 0 || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (size_t i = 0; i < node.num_outputs(); ++i) {
+    const auto& next = node.next_edge(i).function;
+    if (!next || !wanted[i]) continue;
+    const auto stream = next->stream();
+    if (stream.has_value() && stream->id() == 0)
+      fail(std::string(what) + ": the captured backward pass would run on into an eager graph on the default stream (" + next->name() + "): capture all of the graph or detach");
+  }
+}
+
 struct NormBackward : public Node {
   SavedVariable x, residual, weight, seed;
   Tensor stats;
@@ -255,6 +269,7 @@ struct NormBackward : public Node {
     if (c10::GradMode::is_enabled())             // create_graph: a result without a graph would drop the second derivatives in silence
       fail("the gradients of layer_norm and dropout_add_layer_norm are not differentiable (create_graph=True)");
     if (!grads[0].defined()) return variable_list(4);
+    refuse_captured_into_eager("norm_backward", *this, {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2), task_should_compute_output(3)});
     const Tensor tx = x.unpack(), tr = residual.unpack(), tw = weight.unpack(), ts = seed.unpack();
     // hooks on saved tensors may return anything; the kernels take every size and type from x and residual, and the statistics from the forward pass
     const Tensor& dy = grads[0];
@@ -291,6 +306,7 @@ struct DropoutBackward : public Node {
   variable_list apply(variable_list&& grads) override {
     const std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return variable_list(1);
+    refuse_captured_into_eager("dropout_backward", *this, {task_should_compute_output(0)});
     Drop d = drop;
     d.seed_dev = seed.unpack();
     if (d.seed_dev.defined()) check_seed("dropout_backward", d.seed_dev, grads[0].device());

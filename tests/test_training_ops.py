@@ -1181,3 +1181,33 @@ def test_inside_a_compiled_function():
         y = f(*t)
         results.append([y.detach(), *torch.autograd.grad(y, t, o["dy"])])
     assert all(torch.equal(p, q) for p, q in zip(*results))
+
+
+@gpu
+@pytest.mark.parametrize("op", [lambda t: layer_norm(t), lambda t: dropout(t, 0.5, 1), lambda t: dropout_add_layer_norm(t.detach(), t, p=0.5, seed=2)],
+                         ids=["layer_norm", "dropout", "join"])
+def test_captured_backward_into_an_eager_graph_is_refused(op):
+    """x is the result of an eager operation on the default stream: a captured backward pass would make that stream wait inside the capture.  Captured
+    without its backward pass, or with all of the graph inside, it runs."""
+    leaf = torch.randn(4, 32, device="cuda").requires_grad_()
+    x = leaf * 2
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = op(x)
+        with pytest.raises(hip.HipError, match="eager graph"):
+            torch.autograd.grad(y, leaf, torch.ones_like(y))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y.detach(), op(x.detach()))
+    del x, y
+    torch.cuda.synchronize()
+    inside = leaf.detach().clone().requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = op(inside * 2)
+        d, = torch.autograd.grad(y, inside, torch.ones_like(y))
+    graph.replay()
+    torch.cuda.synchronize()
+    y = op(leaf * 2)
+    assert torch.equal(d, torch.autograd.grad(y, leaf, torch.ones_like(y))[0])
