@@ -1211,3 +1211,15 @@ def test_captured_backward_into_an_eager_graph_is_refused(op):
     torch.cuda.synchronize()
     y = op(leaf * 2)
     assert torch.equal(d, torch.autograd.grad(y, leaf, torch.ones_like(y))[0])
+
+
+@gpu
+@pytest.mark.parametrize("cols", [3, 1030, 1700, 2051, 8200, 16384, 17001])
+def test_norm_without_rows(cols):
+    """Every kernel's form of no work at all: empty results, zeros as the parameters' gradients."""
+    for types in ((F32, None, F32), (F16, None, F16), (BF16, F32, F32)):
+        o = operands((0, cols), *types, "both", seed=cols)
+        _, grads = check(o, p=0.2, seed=1)
+        assert not grads["weight"].any() and not grads["bias"].any()
+    x = torch.zeros(2, 0, cols, device="cuda", requires_grad=True)
+    assert layer_norm(x).shape == (2, 0, cols) and dropout(x, 0.5, 1).shape == (2, 0, cols)
